@@ -399,6 +399,92 @@ XG_API int xg_build_label_rows(int32_t labels, const int64_t* token_off, const i
                                int64_t* row_offsets, int32_t* row_tokens, int32_t* row_owners,
                                int32_t* rows, int64_t* tokens, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Beam search (no counterpart in the reference, whose engine masks logits and leaves
+ * decoding to its caller): selection over beams and vocabulary, reordering of per-beam
+ * state, and the back-trace.  A batch holds `groups` requests of `beams` beams each (1 to
+ * XG_MAX_BEAMS); row r = group * beams + beam.  The functions below without an engine work
+ * on the current device; all are asynchronous on `stream`, allocate nothing and may be
+ * captured into a graph. */
+#define XG_MAX_BEAMS 64
+#define XG_MAX_CANDIDATES 128
+#define XG_MAX_BEAM_VOCAB (1 << 20)
+
+/* Bytes of workspace that a selection of these sizes needs on the current device (16-byte
+ * aligned; used during the call's kernels only, so calls that may overlap on the GPU, two
+ * captured graphs among them, need one each). */
+XG_API int xg_beam_workspace(int32_t groups, int32_t beams, int32_t vocab, int32_t dtype, int32_t candidates,
+                             int64_t* bytes);
+/* The `candidates` (1 to XG_MAX_CANDIDATES) best continuations of each group.  With x the
+ * logits of row r (dtype, rows row_stride elements apart, `vocab` columns read) and A_r the
+ * tokens v < vocab whose bit of the row's mask is set (mask: uint32 words, rows mask_stride
+ * words apart; null: every token) and whose logit is not -inf, continuing beam b of group g
+ * with token v in A_r scores
+ *     scores[g][b] + x[r][v] - log(sum over N_r of exp(x[r][u]))
+ * with N_r = A_r (renormalize != 0: the constrained distribution) or every u < vocab (the
+ * model's own).  A finished beam (finished, uint8 [groups][beams], may be null) offers one
+ * continuation, end_token, at its own score, and its logits are not read.  Candidates come
+ * best first, equal scores by the lower (beam, token); out_finished says that the beam was
+ * finished or the token is end_token (-1: none; required with finished).  Rows that offer
+ * nothing: a score that is not finite (-inf marks an empty beam), nothing in A_r, or a sum
+ * that is not finite (a NaN or +inf logit in N_r).  Places left over hold score -inf, beam
+ * and token -1.  A candidate's float32 score is rounded once from 64 bits; the order is by
+ * 64-bit scores, whose log-sum is taken again in 64 bits where two beams' candidates lie
+ * within the 32-bit sum's error of each other. */
+XG_API int xg_beam_select(const void* logits, int32_t dtype, int32_t groups, int32_t beams, int32_t vocab,
+                          int64_t row_stride, const float* scores, const uint32_t* mask, int64_t mask_stride,
+                          const uint8_t* finished, int32_t candidates, int32_t end_token, int32_t renormalize,
+                          float* out_scores, int32_t* out_beams, int32_t* out_tokens, uint8_t* out_finished,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+/* xg_beam_select under the engine's own masks, read in place (nothing is written into the
+ * logits): row r belongs to slots[r] (device int32 [groups * beams]); rows of inactive slots
+ * and of slots in the error phase take every token < vocab, as apply_mask leaves them.
+ * XG_EINVAL for an engine with a logit policy (release or escape bias), whose rows only
+ * xg_apply_mask and the fused step produce. */
+XG_API int xg_engine_beam_select(XgEngine* engine, const void* logits, int32_t dtype, int32_t groups, int32_t beams,
+                                 int32_t cols, int64_t row_stride, const int32_t* slots, const float* scores,
+                                 const uint8_t* finished, int32_t candidates, int32_t end_token, int32_t renormalize,
+                                 float* out_scores, int32_t* out_beams, int32_t* out_tokens, uint8_t* out_finished,
+                                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A tensor of per-row state: `rows` rows, row_stride elements apart, each of up to four
+ * dimensions (size, stride in elements; trailing entries past `dims` unused) of
+ * element_bytes (1, 2, 4, 8 or 16) each.  position_dim: the dimension that `lengths` of
+ * xg_beam_reorder counts (-1: none, whole rows move). */
+typedef struct XgRowTensor {
+  void* data;
+  int64_t rows, row_stride;
+  int64_t size[4], stride[4];
+  int32_t dims, element_bytes, position_dim, reserved;
+} XgRowTensor;
+
+/* In place, for every tensor: row rows[g][b] takes what row rows[g][parents[g][b]] held
+ * before the call (rows, device int32 [groups][beams] of distinct row numbers, or null: row
+ * g * beams + b), at positions below lengths[g] of the tensor's position_dim (lengths:
+ * device int32 [groups], or null: whole rows); every other position keeps its value.  A
+ * parent outside [0, beams) leaves its row as it is, and so does a row number outside the
+ * tensor.  Tensors must not overlap one another or themselves; the host descriptors are
+ * read before the call returns. */
+XG_API int xg_beam_reorder(const XgRowTensor* tensors, int32_t count, const int32_t* parents, int32_t groups,
+                           int32_t beams, const int32_t* lengths, const int32_t* rows, void* stream);
+/* The same for the engine's slots: slots[g][b] takes the whole state of slots[g][parents[g][b]]
+ * (span state, slot memory with its frontier and KG version, recorded mask, history cursor,
+ * activity, STOP table).  slots: device int32 [groups][beams], distinct; entries outside the
+ * engine's slots are skipped. */
+XG_API int xg_reorder_slots(XgEngine* engine, const int32_t* slots, const int32_t* parents, int32_t groups,
+                            int32_t beams, void* stream);
+
+/* The sequences that a search wrote: step t gave place k of group g the token
+ * tokens[t][g][k] on top of place parents[t][g][k] of step t - 1 (int32 traces, step and
+ * group strides in elements, the beams of a group contiguous).  out int32
+ * [groups][beams][steps] (contiguous): out[g][k][t] for t < lengths[g] (device int32
+ * [groups], clamped to [0, steps]; null: steps) is the token of step t on the way to place
+ * k of the group's last step, pad from lengths[g] on and before a parent outside
+ * [0, beams). */
+XG_API int xg_beam_sequences(const int32_t* tokens, int64_t token_step, int64_t token_group, const int32_t* parents,
+                             int64_t parent_step, int64_t parent_group, int32_t steps, int32_t groups, int32_t beams,
+                             const int32_t* lengths, int32_t pad, int32_t* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

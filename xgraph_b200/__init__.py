@@ -27,6 +27,10 @@ _EXPORTS = {
     "SpanSyntax": "syntax",
     "MatchedExecutor": "programs",
     "MatchedPath": "programs",
+    "BeamCandidates": "beams",
+    "beam_reorder": "beams",
+    "beam_select": "beams",
+    "beam_sequences": "beams",
 }
 __all__ = list(_EXPORTS)
 

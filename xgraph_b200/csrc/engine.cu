@@ -21,6 +21,7 @@
 #include <string>
 #include <vector>
 
+#include "beams.h"
 #include "core.cuh"
 
 namespace xg {
@@ -192,6 +193,15 @@ __global__ void fill_kernel(const __grid_constant__ Tables t) {
     t.base[slot] = nullptr;
     t.delta[slot] = own;
   }
+}
+
+// After slots were reordered: a slot's own mask bits are in its own buffer row.
+__global__ void relink_kernel(const __grid_constant__ Tables t, const int32_t* slots, int32_t count, int32_t max_slots) {
+  const int32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= count) return;
+  const int32_t slot = slots[i];
+  if (slot < 0 || slot >= max_slots) return;
+  if (t.delta[slot]) t.delta[slot] = t.masks + static_cast<int64_t>(slot) * t.words_padded;
 }
 
 __device__ __forceinline__ uint32_t mask_word(const uint32_t* base, const uint32_t* delta, int64_t w) {
@@ -2593,6 +2603,84 @@ int xg_apply_mask_noalloc(XgEngine* e, void* logits, int32_t dtype, int32_t rows
   if (int rc = noalloc_scratch(device, &scratch)) return rc;
   return launch_drafts(e, data_of(logits), dtype, rows, cols, row_stride, row_slots, local_pos, input_ids, scratch,
                        stream);
+}
+
+int xg_engine_beam_select(XgEngine* e, const void* logits, int32_t dtype, int32_t groups, int32_t beams, int32_t cols,
+                          int64_t row_stride, const int32_t* slots, const float* scores, const uint8_t* finished,
+                          int32_t candidates, int32_t end_token, int32_t renormalize, float* out_scores,
+                          int32_t* out_beams, int32_t* out_tokens, uint8_t* out_finished, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  if (!e) return fail(XG_EINVAL, "null engine");
+  if (e->t.release_on || e->t.escape_bias != 0.0f)
+    return fail(XG_EINVAL, "beam selection reads the slots' masks, which a logit policy (release, escape bias) does not "
+                           "change: apply_mask the logits, then select without masks");
+  if (groups > 0 && !slots) return fail(XG_EINVAL, "null argument");
+  if (row_stride < cols) return fail(XG_EINVAL, "logits need one contiguous row per beam");
+  beams::SelectArgs a{};
+  a.logits = static_cast<const char*>(logits);
+  a.row_stride = row_stride;
+  a.dtype = dtype;
+  a.groups = groups;
+  a.beams = beams;
+  a.vocab = cols < e->layout.vocab ? cols : e->layout.vocab;
+  a.candidates = candidates;
+  a.end_token = end_token;
+  a.renormalize = renormalize != 0;
+  a.scores = scores;
+  a.finished = finished;
+  a.masks.slots = slots;
+  a.masks.base = e->t.base;
+  a.masks.delta = e->t.delta;
+  a.masks.active = e->t.active;
+  a.masks.max_slots = e->max_sequences;
+  a.out_scores = out_scores;
+  a.out_beams = out_beams;
+  a.out_tokens = out_tokens;
+  a.out_finished = out_finished;
+  a.workspace = static_cast<char*>(workspace);
+  a.workspace_bytes = workspace_bytes;
+  return beams::select(a, as_stream(stream));
+}
+
+int xg_reorder_slots(XgEngine* e, const int32_t* slots, const int32_t* parents, int32_t groups, int32_t beams,
+                     void* stream) {
+  if (!e) return fail(XG_EINVAL, "null engine");
+  if (groups < 0 || beams < 1 || static_cast<int64_t>(groups) * beams > e->max_sequences)
+    return fail(XG_EINVAL, "more slots than max_sequences");
+  if (groups == 0) return XG_OK;
+  if (!slots || !parents) return fail(XG_EINVAL, "null argument");
+  XgRowTensor moved[12];
+  int32_t count = 0;
+  auto add = [&](const void* data, int64_t words) {  // one row of 32-bit words per slot
+    XgRowTensor t{};
+    t.data = const_cast<void*>(data);
+    t.rows = e->max_sequences;
+    t.row_stride = words;
+    t.size[0] = words;
+    t.stride[0] = 1;
+    t.dims = 1;
+    t.element_bytes = 4;
+    t.position_dim = -1;
+    moved[count++] = t;
+  };
+  add(e->states, XG_STATE_INTS);
+  add(e->memory, e->t.memory_ints);
+  add(e->masks, e->layout.words_padded);
+  add(e->base, sizeof(uint32_t*) / 4);
+  add(e->delta, sizeof(uint32_t*) / 4);
+  add(e->cursors, 1);
+  add(e->active, 1);
+  if (e->stop_on) {
+    add(e->stop_on, 1);
+    add(e->stop_rel, static_cast<int64_t>(e->t.relations) * 3);
+    add(e->stop_woff, kMaxStopWords + 2);
+    add(e->stop_words, kMaxStopBytes / 4);
+  }
+  if (int rc = beams::reorder(moved, count, parents, groups, beams, nullptr, slots, as_stream(stream))) return rc;
+  const int32_t n = groups * beams;
+  relink_kernel<<<static_cast<unsigned>((n + 127) / 128), 128, 0, as_stream(stream)>>>(e->t, slots, n, e->max_sequences);
+  XG_CUDA(cudaGetLastError(), "slot relink kernel");
+  return XG_OK;
 }
 
 }  // extern "C"

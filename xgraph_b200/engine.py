@@ -118,6 +118,14 @@ def load_library(path: Path = LIBRARY):
         "xg_set_expressions": ([p, p, i64, i32, p, p, p, i32, p], ctypes.c_int),
         "xg_build_label_rows": ([i32, p, p, i64, p, p, i64, p, i32, i32, p, p, i64, p, p, p, p, p, p, p, p],
                                 ctypes.c_int),
+        "xg_beam_workspace": ([i32, i32, i32, i32, i32, ctypes.POINTER(i64)], ctypes.c_int),
+        "xg_beam_select": ([p, i32, i32, i32, i32, i64, p, p, i64, p, i32, i32, i32, p, p, p, p, p, i64, p],
+                           ctypes.c_int),
+        "xg_engine_beam_select": ([p, p, i32, i32, i32, i32, i64, p, p, p, i32, i32, i32, p, p, p, p, p, i64, p],
+                                  ctypes.c_int),
+        "xg_beam_reorder": ([p, i32, p, i32, i32, p, p, p], ctypes.c_int),
+        "xg_reorder_slots": ([p, p, p, i32, i32, p], ctypes.c_int),
+        "xg_beam_sequences": ([p, i64, i64, p, i64, i64, i32, i32, i32, p, i32, p, p], ctypes.c_int),
     }
     for name, (args, res) in sigs.items():
         fn = getattr(lib, name)
@@ -626,6 +634,46 @@ class Engine:
         _check(self._lib.xg_apply_mask(
             self._handle, ctypes.c_void_p(logits.data_ptr()), dtype, n, logits.shape[1],
             logits.stride(0) if n > 1 else logits.shape[1], ptr, drafts[0], drafts[1], _stream(stream)))
+
+    def beam_select(self, logits, slots, scores, *, finished=None, candidates: int | None = None,
+                    end_token: int | None = None, renormalize: bool = True, stream: int = 0):
+        """beams.beam_select under the slots' masks, read in place: row (group, b) of logits is
+        constrained by slots[group, b] (int32 [groups, beams]) as apply_mask would mask it, and
+        the logits are not written.  Rows of inactive slots and error rows take any token of
+        the served vocabulary.  Not for an engine with a logit policy (release, escape bias):
+        apply_mask its logits, then beams.beam_select without a mask."""
+        from . import beams as _beams
+
+        torch = _beams._load()
+        if not isinstance(scores, torch.Tensor) or scores.dim() != 2:
+            raise ValueError("scores must be [groups, beams]")
+        if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 2:
+            raise ValueError("logits must be a 2-D tensor on the GPU")
+        if logits.device.index != self._info.device:
+            raise ValueError(f"logits must be on the engine's GPU (cuda:{self._info.device})")
+        slots_at = _beams._table(slots, "slots", tuple(scores.shape), torch.int32, logits.device)
+        return _beams._select(self._handle, logits, slots_at, scores, None, finished, candidates,
+                              min(logits.shape[1], self.vocab_size), end_token, renormalize, stream)
+
+    def reorder(self, slots, beams, stream: int = 0) -> None:
+        """After a beam selection: slots[group, b] takes the whole constraint state of
+        slots[group, beams[group, b]] (span state, memory, KG version, recorded mask, history
+        cursor, STOP table).  Both int32 [groups, beams]; slots distinct; an entry of beams
+        outside [0, beams) leaves its slot as it is.  The next sync reads each slot's history
+        from the cursor it took over, so a slot's history row needs its new tokens only."""
+        import torch
+
+        for name, table in (("slots", slots), ("beams", beams)):
+            if (not isinstance(table, torch.Tensor) or not table.is_cuda or table.dtype != torch.int32
+                    or table.dim() != 2 or not table.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous [groups, beams] int32 tensor on the GPU")
+        if slots.shape != beams.shape:
+            raise ValueError("slots and beams must have the same shape")
+        if slots.numel() > self.max_sequences:
+            raise ValueError("more slots than max_sequences")
+        _check(self._lib.xg_reorder_slots(self._handle, ctypes.c_void_p(slots.data_ptr()),
+                                          ctypes.c_void_p(beams.data_ptr()), slots.shape[0], slots.shape[1],
+                                          _stream(stream)))
 
     def _row_slots(self, row_slots, name="row_slots"):
         import torch
