@@ -7,6 +7,7 @@
 #include <math_constants.h>
 
 #include <atomic>
+#include <cfloat>
 #include <string>
 
 extern "C" int xg_set_error(int code, const char* message);
@@ -20,14 +21,22 @@ constexpr uint32_t kFull = 0xffffffffu;
 // ---------------------------------------------------------------------------------------
 // Selection, first kernel: every row's log-sum parts and its best tokens.
 //
-// A CTA streams a share of one row in tiles that stay in registers (kVecs 16-byte loads a
-// thread, all in flight together), so each logit is read once: the tile's maximum and sum of
-// exponentials, then its candidates, come from the same registers.
+// A CTA streams a share of one row in steps of kVecs 16-byte vectors a thread.  The vectors go
+// through a ring in shared memory that each thread fills (cp.async, two steps ahead) and reads
+// for itself, so loads stay in flight while a step is computed on and no register holds them.
+// Each logit is read once: a step adds its exponentials to the thread's sum and leaves the
+// maximum of the thread's vectors in shared memory.  The best tokens lie in the few entries of
+// that table whose maximum is among its best; those alone are read again for their tokens.
 
 constexpr int32_t kScanThreads = 256;
 constexpr int32_t kScanWarps = kScanThreads / 32;
-constexpr int32_t kVecs = 8;          // 16-byte vectors a thread holds of a tile
-constexpr int32_t kPushCap = 1024;    // candidates a tile may offer before the exact search takes over
+constexpr int32_t kVecs = 4;          // 16-byte vectors of a thread in one step: an entry of the table
+constexpr int32_t kSteps = 2;         // steps in the ring
+constexpr int32_t kRound = 16;        // steps of the table; after as many the best tokens are taken out
+constexpr int32_t kListCap = 512;     // entries read again; see list_crowded for why they suffice
+constexpr int32_t kPushCap = 1024;    // tokens (keys) of the listed entries
+constexpr int32_t kRankMost = kScanThreads;  // keys put in order by counting
+constexpr float kFar = 65536.0f;
 constexpr int32_t kPoolMax = 8192;    // candidates of a group that the second kernel takes
 
 // Floats as unsigned integers of the same order (-0 made +0 by the caller).
@@ -76,8 +85,13 @@ struct F32 {
   __device__ static float at(const uint4& v, int k) { return __uint_as_float((&v.x)[k]); }
   __device__ static float one(const char* p) { return *reinterpret_cast<const float*>(p); }
   __device__ static void put(uint4& v, int k, const char* p) { (&v.x)[k] = *reinterpret_cast<const uint32_t*>(p); }
-  __device__ static float top(const uint4& v) {
-    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+  __device__ static float top(const uint4 (&v)[kVecs]) {
+    float m = __uint_as_float(v[0].x);
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j)
+      m = max_nan(max_nan(m, __uint_as_float(v[j].x)),
+                  max_nan(max_nan(__uint_as_float(v[j].y), __uint_as_float(v[j].z)), __uint_as_float(v[j].w)));
+    return m;
   }
   __device__ static void keep(uint4& v, uint32_t bits) {
     v.x = (bits & 1u) ? v.x : kNegInf;
@@ -113,9 +127,12 @@ struct BF16 : Half<0xff80u> {
   __device__ static float one(const char* p) {
     return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << 16);
   }
-  __device__ static float top(const uint4& v) {
+  __device__ static float top(const uint4 (&v)[kVecs]) {
     const auto h = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
-    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h(v.x), h(v.y)), __hmax2_nan(h(v.z), h(v.w)));
+    __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h(v[0].x), h(v[0].y)), __hmax2_nan(h(v[0].z), h(v[0].w)));
+#pragma unroll
+    for (int j = 1; j < kVecs; ++j)
+      m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(h(v[j].x), h(v[j].y)), __hmax2_nan(h(v[j].z), h(v[j].w))));
     return max_nan(__low2float(m), __high2float(m));
   }
 };
@@ -127,9 +144,12 @@ struct F16 : Half<0xfc00u> {
   __device__ static float one(const char* p) {
     return __half2float(__ushort_as_half(*reinterpret_cast<const unsigned short*>(p)));
   }
-  __device__ static float top(const uint4& v) {
+  __device__ static float top(const uint4 (&v)[kVecs]) {
     const auto h = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
-    const __half2 m = __hmax2_nan(__hmax2_nan(h(v.x), h(v.y)), __hmax2_nan(h(v.z), h(v.w)));
+    __half2 m = __hmax2_nan(__hmax2_nan(h(v[0].x), h(v[0].y)), __hmax2_nan(h(v[0].z), h(v[0].w)));
+#pragma unroll
+    for (int j = 1; j < kVecs; ++j)
+      m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(h(v[j].x), h(v[j].y)), __hmax2_nan(h(v[j].z), h(v[j].w))));
     return max_nan(__low2float(m), __high2float(m));
   }
 };
@@ -163,12 +183,13 @@ __device__ __forceinline__ RowMask row_mask(const RowMasks& m, int32_t row) {
   return RowMask{m.words ? m.words + row * m.stride : nullptr, nullptr};
 }
 
-// What the scan leaves for the merge: per (row, share) the log-sum parts, and its best keys,
-// best first (rising(logit) << 32 | ~token; 0: none).
+// What the scan leaves for the merge: per (row, share) the sum's parts, and its best keys, best
+// first (rising(logit) << 32 | ~token; 0: none).
 struct Part {
-  double sum;  // of exp(x - top)
-  float top;
-  int32_t pad;
+  double sum;      // of 2^(x log2 e - anchor)
+  double far_sum;  // of exp(x - far), from tiles whose maximum is far from 0
+  float anchor;    // a whole number; -inf: no sum
+  float far;       // -inf: no far sum
 };
 
 struct ScanArgs {
@@ -183,6 +204,11 @@ __device__ __forceinline__ uint64_t make_key(uint32_t order, int32_t token) {
   return (static_cast<uint64_t>(order) << 32) | static_cast<uint32_t>(~token);
 }
 
+// 2^k of a whole number k <= 0 (0 below the normal doubles), exactly.
+__device__ __forceinline__ double power2(float k) {
+  return k < -1000.0f ? 0.0 : __hiloint2double((1023 + static_cast<int32_t>(k)) << 20, 0);
+}
+
 // Row r takes part: its score is finite and the beam has not ended.
 __device__ __forceinline__ bool row_scans(const SelectArgs& a, int32_t row) {
   const bool ended = a.finished && a.finished[row];
@@ -190,14 +216,19 @@ __device__ __forceinline__ bool row_scans(const SelectArgs& a, int32_t row) {
 }
 
 struct ScanShared {
-  uint64_t pushed[kPushCap];
-  uint64_t best[2][kMaxCandidates];
-  uint32_t group_top[kMaxCandidates];  // the maxima of the groups a tile's threads form
-  double warp_sum[kScanWarps];
-  float warp_top[kScanWarps];
+  uint4 ring[kSteps * kVecs * kScanThreads];  // afterwards the listed entries' vectors
+  union {
+    uint32_t tops[kRound][kScanThreads];  // rising() of each thread's maximum in each step
+    uint64_t pushed[kPushCap];            // afterwards the listed entries' keys
+  };
+  uint64_t few[kRankMost];
+  int32_t list[kListCap];              // entries: step of the round * kScanThreads + thread
+  uint32_t thread_top[kScanThreads];   // the threads' maxima in the round
+  Part warp_part[kScanWarps];
   int32_t counts[2][kScanWarps];
-  int32_t count;
+  int32_t listed, count, few_count;
 };
+static_assert(kListCap * kVecs <= kSteps * kVecs * kScanThreads, "the ring holds the listed vectors");
 
 __device__ __forceinline__ int32_t block_total(int32_t mine, int32_t (&counts)[kScanWarps]) {
   const int32_t of_warp = __reduce_add_sync(kFull, mine);
@@ -209,91 +240,340 @@ __device__ __forceinline__ int32_t block_total(int32_t mine, int32_t (&counts)[k
   return total;
 }
 
+// The best min(n, wanted) of the n keys in sh.pushed, in order, into sh.few (all threads; a
+// barrier before the call has made the keys visible and one is passed after them).
+__device__ __forceinline__ int32_t best_of(ScanShared& sh, int32_t n, int32_t wanted) {
+  const int32_t tid = threadIdx.x;
+  constexpr int32_t kEach = kPushCap / kScanThreads;
+  uint64_t edge = 0;
+  if (n > kRankMost) {  // fewer first: bisect the keys until at most kRankMost are above the edge
+    uint64_t key[kEach];
+#pragma unroll
+    for (int32_t i = 0; i < kEach; ++i) key[i] = tid + i * kScanThreads < n ? sh.pushed[tid + i * kScanThreads] : 0u;
+    int32_t turn = 0;
+    for (int32_t bit = 63; bit >= 0; --bit, turn ^= 1) {
+      const uint64_t trial = edge | (1ull << bit);
+      int32_t mine = 0;
+#pragma unroll
+      for (int32_t i = 0; i < kEach; ++i) mine += key[i] >= trial;
+      const int32_t total = block_total(mine, sh.counts[turn]);
+      if (total >= wanted) {
+        edge = trial;
+        if (total <= kRankMost) break;
+      }
+    }
+    __syncthreads();
+    if (tid == 0) sh.few_count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int32_t i = 0; i < kEach; ++i)
+      if (key[i] >= edge && key[i] != 0u) sh.few[atomicAdd(&sh.few_count, 1)] = key[i];
+    __syncthreads();
+    n = sh.few_count;
+    for (int32_t i = tid; i < n; i += kScanThreads) sh.pushed[i] = sh.few[i];
+    __syncthreads();
+  }
+  uint64_t mine = 0;
+  int32_t rank = kRankMost;
+  if (tid < n) {
+    mine = sh.pushed[tid];
+    rank = 0;
+#pragma unroll 4
+    for (int32_t j = 0; j < n; ++j) rank += sh.pushed[j] > mine;
+  }
+  if (rank < wanted) sh.few[rank] = mine;
+  __syncthreads();
+  return min(n, wanted);
+}
+
+// Where an entry's vector j begins: entry = step of the round * kScanThreads + thread, and
+// `first` the token of the round's first vector (a warp's vectors of a step are consecutive).
+template <typename E>
+__device__ __forceinline__ int32_t vector_token(int32_t entry, int32_t j, int32_t first) {
+  const int32_t step = entry / kScanThreads, thread = entry % kScanThreads;
+  return first + (((step * kScanWarps + thread / 32) * kVecs + j) * 32 + thread % 32) * E::kPer;
+}
+
+// More than kListCap entries reach the bound (ties, or fewer than `wanted` threads saw a token):
+// the bound rises by bisection until at most kRankMost do.  Where equal maxima do not let it,
+// the entries above it are taken and, of those at it, the ones of the earliest steps that hold
+// `wanted` together: a later step's equal tokens come after theirs.  That is fewer than
+// 2 * wanted + kScanThreads <= kListCap entries.  Returns the bound.
+__device__ __noinline__ uint32_t list_crowded(ScanShared& sh, int32_t steps, int32_t wanted) {
+  const int32_t tid = threadIdx.x;
+  int32_t turn = 0;
+  const auto count_if = [&](auto pick) {
+    int32_t mine = 0;
+#pragma unroll 1
+    for (int32_t step = 0; step < steps; ++step) mine += pick(sh.tops[step][tid], step);
+    turn ^= 1;
+    return block_total(mine, sh.counts[turn]);
+  };
+  uint32_t edge = 0;
+  int32_t level = 0x7fffffff, last = kRound;  // entries at the edge are taken up to step `last`
+  for (int32_t bit = 31; bit >= 0 && level > kRankMost; --bit) {
+    const uint32_t trial = edge | (1u << bit);
+    const int32_t total = count_if([=](uint32_t o, int32_t) { return o >= trial; });
+    if (total >= wanted) {
+      edge = trial;
+      level = total;
+    }
+  }
+  if (level > kRankMost) {
+    const int32_t above = count_if([=](uint32_t o, int32_t) { return o > edge; });
+    for (last = 0; last < steps; ++last)
+      if (count_if([=](uint32_t o, int32_t step) { return o == edge && step <= last; }) >= wanted - above) break;
+  }
+  edge = max(edge, kRisingLowest);
+  __syncthreads();
+  if (tid == 0) sh.listed = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int32_t step = 0; step < steps; ++step) {
+    const uint32_t o = sh.tops[step][tid];
+    if (o >= edge && (o > edge || step <= last)) {
+      const int32_t n = atomicAdd(&sh.listed, 1);
+      if (n < kListCap) sh.list[n] = step * kScanThreads + tid;
+    }
+  }
+  __syncthreads();
+  return edge;
+}
+
+// Too many tokens of the vectors in sh.ring reach the bound: it rises by bisection until at
+// most kRankMost do, and where equal logits do not let it, the lowest tokens are taken.  Their
+// keys, `wanted` to kRankMost, follow the `held` ones in sh.pushed.
+template <typename E>
+__device__ __noinline__ void push_crowded(ScanShared& sh, int32_t vectors, int32_t first, int32_t held, int32_t wanted) {
+  constexpr int32_t kPer = E::kPer;
+  const int32_t tid = threadIdx.x;
+  int32_t turn = 0;
+  const auto count_if = [&](auto pick) {
+    int32_t mine = 0;
+#pragma unroll 1
+    for (int32_t i = tid; i < vectors; i += kScanThreads) {
+      const uint4 v = sh.ring[i];
+      const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
+#pragma unroll
+      for (int32_t k = 0; k < kPer; ++k) mine += pick(rising(E::at(v, k) + 0.0f), t0 + k);
+    }
+    turn ^= 1;
+    return block_total(mine, sh.counts[turn]);
+  };
+  uint32_t edge = 0;
+  int32_t level = 0x7fffffff, last = 0x7fffffff;  // of the tokens equal to the edge, those up to `last`
+  for (int32_t bit = 31; bit >= 0 && level > kRankMost; --bit) {
+    const uint32_t trial = edge | (1u << bit);
+    const int32_t total = count_if([=](uint32_t o, int32_t) { return o >= trial; });
+    if (total >= wanted) {
+      edge = trial;
+      level = total;
+    }
+  }
+  if (level > kRankMost) {
+    const int32_t above = count_if([=](uint32_t o, int32_t) { return o > edge; });
+    last = -1;
+    for (int32_t bit = 20; bit >= 0; --bit) {
+      const int32_t trial = last + (1 << bit);
+      if (count_if([=](uint32_t o, int32_t t) { return o == edge && t <= trial; }) < wanted - above) last = trial;
+    }
+    ++last;
+  }
+  edge = max(edge, kRisingLowest);
+  __syncthreads();
+  if (tid == 0) sh.count = held;
+  __syncthreads();
+#pragma unroll 1
+  for (int32_t i = tid; i < vectors; i += kScanThreads) {
+    const uint4 v = sh.ring[i];
+    const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
+#pragma unroll
+    for (int32_t k = 0; k < kPer; ++k) {
+      const uint32_t o = rising(E::at(v, k) + 0.0f);
+      if (o >= edge && (o > edge || t0 + k <= last)) {
+        const int32_t n = atomicAdd(&sh.count, 1);
+        if (n < kPushCap) sh.pushed[n] = make_key(o, t0 + k);
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// The parts of a warp's lanes as one (in every lane).
+__device__ __forceinline__ Part total_part(Part p) {
+  float anchor = p.anchor;
+#pragma unroll
+  for (int32_t d = 16; d > 0; d >>= 1) anchor = fmaxf(anchor, __shfl_xor_sync(kFull, anchor, d));
+  double sum = p.anchor == -CUDART_INF_F ? 0.0 : p.sum * power2(p.anchor - anchor);
+#pragma unroll
+  for (int32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+  float far = p.far;
+  double far_sum = 0.0;
+  if (__any_sync(kFull, far != -CUDART_INF_F)) {
+#pragma unroll
+    for (int32_t d = 16; d > 0; d >>= 1) far = fmaxf(far, __shfl_xor_sync(kFull, far, d));
+    if (p.far != -CUDART_INF_F) far_sum = p.far_sum * exp(static_cast<double>(p.far) - static_cast<double>(far));
+#pragma unroll
+    for (int32_t d = 16; d > 0; d >>= 1) far_sum += __shfl_xor_sync(kFull, far_sum, d);
+  }
+  return Part{sum, far_sum, anchor, far};
+}
+
+__device__ __forceinline__ void copy_async(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared))),
+               "l"(global)
+               : "memory");
+}
+__device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_async() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One vector of a row: tokens t0 .. t0 + kPer, -inf outside [0, vocab).
+template <typename E>
+__device__ __forceinline__ uint4 load_vector(const char* logits, int32_t t0, int32_t vocab) {
+  const char* at = logits + static_cast<int64_t>(t0) * E::kBytes;
+  if (t0 >= 0 && t0 + E::kPer <= vocab) return *reinterpret_cast<const uint4*>(at);
+  uint4 v = make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
+#pragma unroll
+  for (int32_t k = 0; k < E::kPer; ++k)
+    if (t0 + k >= 0 && t0 + k < vocab) E::put(v, k, at + k * E::kBytes);
+  return v;
+}
+
 template <typename E, bool MASKED, bool RENORMALIZE>
-__global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const __grid_constant__ ScanArgs s) {
-  __shared__ ScanShared sh;
+__global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_constant__ ScanArgs s) {
+  extern __shared__ __align__(16) char dynamic[];
+  ScanShared& sh = *reinterpret_cast<ScanShared*>(dynamic);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge waits for this grid's end
   constexpr int32_t kPer = E::kPer;
-  constexpr int32_t kTileVecs = kScanThreads * kVecs;
+  constexpr int32_t kWarpTokens = 32 * kVecs * kPer;  // a warp's vectors of a step are consecutive
+  constexpr int32_t kStepTokens = kScanWarps * kWarpTokens;
+  constexpr uint32_t kAll = (1u << kPer) - 1u;
+  constexpr bool kSkips = MASKED && RENORMALIZE;  // vectors without an allowed token are not read
+  static_assert(kVecs * kPer <= 32, "a lane's bits of a step fit one word");
   const SelectArgs& a = s.a;
   const int32_t row = blockIdx.x / s.shares, share = blockIdx.x - row * s.shares;
-  if (!row_scans(a, row)) return;
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t wanted = a.candidates, vocab = a.vocab;
+  const bool scans = row_scans(a, row);
   const char* logits = a.logits + static_cast<int64_t>(row) * a.row_stride * E::kBytes;
   // vectors start at 16-byte boundaries, so the first may begin before the row
   const int32_t head = static_cast<int32_t>(reinterpret_cast<uintptr_t>(logits) & 15u) / E::kBytes;
-  const int32_t vecs = (vocab + head + kPer - 1) / kPer;
+  const int32_t begin = share * s.tiles_per_share;
+  const int32_t end = min(begin + s.tiles_per_share, (vocab + head + kStepTokens - 1) / kStepTokens);
+
+  // the warp's first token of a step; a lane's vectors follow one another at 32 vectors' distance
+  const auto warp_token = [&](int32_t step) { return step * kStepTokens + warp * kWarpTokens - head; };
   const RowMask mask = MASKED ? row_mask(a.masks, row) : RowMask{nullptr, nullptr};
-  // candidates need a bound that at least `wanted` of a tile's tokens reach: the least of the
-  // maxima of `groups` groups of threads, with groups >= wanted
-  int32_t groups = kScanWarps;
-  while (groups < wanted) groups <<= 1;
-  const int32_t group_lanes = kScanThreads / groups;
-
-  double sum = 0.0;                       // of this warp's tokens so far, relative to `top`
-  float top = -CUDART_INF_F;
-  int32_t held = 0, which = 0;            // sh.best[which] holds the best so far
-  uint32_t bar = kRisingLowest;           // tokens below it cannot be among the best
-
-  const int32_t tile_end = min((share + 1) * s.tiles_per_share, (vecs + kTileVecs - 1) / kTileVecs);
-  for (int32_t tile = share * s.tiles_per_share; tile < tile_end; ++tile) {
-    const int32_t v0 = tile * kTileVecs + tid;
-    uint4 v[kVecs];
-    uint32_t bits[kVecs];
+  // the mask word that the lane holds of the warp's tokens of a step (aligned rows; tokens past
+  // the row cleared), and from the lanes' words each lane's own bits, kPer a vector
+  const auto load_word = [&](int32_t step) {
+    if (!MASKED || head != 0 || step >= end || lane * 32 >= kWarpTokens) return 0u;
+    const int32_t w = warp_token(step) / 32 + lane, left = vocab - w * 32;
+    if (left <= 0) return 0u;
+    const uint32_t word = mask.all() ? kFull : mask.word(w);
+    return left < 32 ? word & ((1u << left) - 1u) : word;
+  };
+  const auto own_bits = [&](int32_t step, uint32_t word) {
+    uint32_t bits = 0u;
+    if (head == 0) {
 #pragma unroll
-    for (int32_t j = 0; j < kVecs; ++j) {
-      const int32_t t0 = (v0 + j * kScanThreads) * kPer - head;
-      bits[j] = t0 >= vocab ? 0u : MASKED ? mask.bits(t0, kPer, vocab) : RowMask{nullptr, nullptr}.bits(t0, kPer, vocab);
-    }
+      for (int32_t j = 0; j < kVecs; ++j) {
+        const uint32_t got = __shfl_sync(kFull, word, j * kPer + lane * kPer / 32);
+        bits |= ((got >> ((lane * kPer) & 31)) & kAll) << (j * kPer);
+      }
+    } else if (step < end) {
 #pragma unroll
-    for (int32_t j = 0; j < kVecs; ++j) {
-      const int32_t t0 = (v0 + j * kScanThreads) * kPer - head;
-      v[j] = make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
-      if (t0 >= vocab || (RENORMALIZE && bits[j] == 0u)) continue;
-      const char* at = logits + static_cast<int64_t>(t0) * E::kBytes;
-      if (t0 >= 0 && t0 + kPer <= vocab) {
-        v[j] = __ldcs(reinterpret_cast<const uint4*>(at));
-      } else {
-#pragma unroll
-        for (int32_t k = 0; k < kPer; ++k)
-          if (t0 + k >= 0 && t0 + k < vocab) E::put(v[j], k, at + k * E::kBytes);
+      for (int32_t j = 0; j < kVecs; ++j) {
+        const int32_t t0 = warp_token(step) + (j * 32 + lane) * kPer;
+        if (t0 < vocab) bits |= mask.bits(t0, kPer, vocab) << (j * kPer);
       }
     }
-    if (MASKED && RENORMALIZE) {
+    return bits;
+  };
+  // the loads of a step into the ring (`to`: the thread's first slot)
+  const auto issue = [&](int32_t step, uint32_t bits, uint4* to) {
+    const int32_t t0 = warp_token(step);
+    if (t0 >= 0 && t0 + kWarpTokens <= vocab) {  // uniform in the warp
+      const char* from = logits + static_cast<int64_t>(t0) * E::kBytes + lane * 16;
 #pragma unroll
-      for (int32_t j = 0; j < kVecs; ++j)
-        if (bits[j] != (1u << kPer) - 1u) E::keep(v[j], bits[j]);
+      for (int32_t j = 0; j < kVecs; ++j) {
+        if (!kSkips || ((bits >> (j * kPer)) & kAll))
+          copy_async(to + j * kScanThreads, from + j * 512);
+        else
+          to[j * kScanThreads] = make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
+      }
+    } else {
+#pragma unroll
+      for (int32_t j = 0; j < kVecs; ++j) {
+        const int32_t t = t0 + (j * 32 + lane) * kPer;
+        if (t < vocab && (!kSkips || ((bits >> (j * kPer)) & kAll)))
+          to[j * kScanThreads] = load_vector<E>(logits, t, vocab);
+        else
+          to[j * kScanThreads] = make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
+      }
     }
-    // the tile's maximum and sum, per warp: exp(x - m) as 2^(x log2 e - a) with a the float
-    // nearest m log2 e, so that the shared part of every exponent is exact
-    float most = E::top(v[0]);
+  };
+
+  double sum = 0.0, far_sum = 0.0;  // this thread's, relative to the warp's anchor and far
+  float anchor = -CUDART_INF_F, far = -CUDART_INF_F;
+  float limit = -CUDART_INF_F;      // logits above it raise the anchor
+  int32_t held = 0;                 // best keys of earlier rounds, in sh.few
+
+  for (int32_t round = begin; round < end; round += kRound) {
+    const int32_t stop = min(round + kRound, end);
+    uint32_t bits[kSteps] = {0u, 0u}, word = 0u;
+    if (MASKED) {
+      if (!scans) return;
+      const uint32_t word0 = load_word(round), word1 = round + 1 < stop ? load_word(round + 1) : 0u;
+      word = round + 2 < stop ? load_word(round + 2) : 0u;
+      bits[0] = own_bits(round, word0);
+      bits[1] = own_bits(round + 1, word1);
+    }
+    issue(round, bits[0], sh.ring + tid);
+    commit_async();
+    if (round + 1 < stop) issue(round + 1, bits[1], sh.ring + kVecs * kScanThreads + tid);
+    commit_async();
+    if (!MASKED && !scans) {  // the first loads did not wait for the row's flags
+      wait_async<0>();
+      return;
+    }
+    float best = -CUDART_INF_F;  // the thread's best logit that it may take
+    for (int32_t step = round; step < stop; ++step) {
+      wait_async<kSteps - 1>();
+      const int32_t at = step - round;
+      uint4* slot = sh.ring + (at & 1) * kVecs * kScanThreads + tid;
+      const uint32_t own = MASKED ? bits[0] : 0u;
+      uint4 v[kVecs];
 #pragma unroll
-    for (int32_t j = 1; j < kVecs; ++j) most = max_nan(most, E::top(v[j]));
-    float shown = most;
-#pragma unroll
-    for (int32_t d = 16; d > 0; d >>= 1) most = max_nan(most, __shfl_xor_sync(kFull, most, d));
-    if (most != -CUDART_INF_F) {  // uniform in the warp
-      double part;
-      if (fabsf(most) < 65536.0f) {
-        const float anchor = __fmul_rn(most, kLog2eHi);
-        const uint64_t hi = pack2(kLog2eHi, kLog2eHi), lo = pack2(kLog2eLo, kLog2eLo), back = pack2(-anchor, -anchor);
-        uint64_t acc[2] = {0, 0};
-#pragma unroll
-        for (int32_t j = 0; j < kVecs; ++j) {
-#pragma unroll
-          for (int32_t k = 0; k < kPer; k += 2) {
-            const uint64_t x = pack2(E::at(v[j], k), E::at(v[j], k + 1));
-            const uint64_t y = fma2(x, lo, fma2(x, hi, back));
-            acc[(k >> 1) & 1] = add2(acc[(k >> 1) & 1], pack2(exp2_fast(low(y)), exp2_fast(high(y))));
-          }
+      for (int32_t j = 0; j < kVecs; ++j) {
+        v[j] = slot[j * kScanThreads];
+        if (kSkips) {
+          const uint32_t b = (own >> (j * kPer)) & kAll;
+          if (b != kAll) E::keep(v[j], b);
         }
-        const uint64_t all = add2(acc[0], acc[1]);
-        part = static_cast<double>(low(all)) + static_cast<double>(high(all));
-#pragma unroll
-        for (int32_t d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(kFull, part, d);
-        part *= exp(static_cast<double>(anchor) * 0.69314718055994530942 - static_cast<double>(most));
-      } else {  // far from 0 (or not finite) the difference comes first
+      }
+      float shown = E::top(v);
+      bool far_step = false;
+      if (__any_sync(kFull, !(shown <= limit))) {  // the first tokens, or a new maximum, or a NaN
+        const float most = from_rising(__reduce_max_sync(kFull, rising(shown)));
+        if (!isfinite(most)) {
+          if (anchor == -CUDART_INF_F) anchor = 0.0f;  // whatever the anchor, the sum will show it
+        } else if (fabsf(most) < kFar) {
+          const float near = ceilf(most * kLog2eHi);
+          if (near > anchor) {
+            sum = anchor == -CUDART_INF_F ? 0.0 : sum * power2(anchor - near);
+            anchor = near;
+            limit = near * 0.693147f;
+          }
+        } else {
+          far_step = true;
+        }
+      }
+      if (far_step) {  // so far from 0 that log2 e's rounding would show: the difference comes first
+        const float most = from_rising(__reduce_max_sync(kFull, rising(shown)));
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int32_t j = 0; j < kVecs; ++j) {
@@ -303,140 +583,122 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const __grid_cons
             acc[k & 3] += exp2_fast(fmaf(d, kLog2eHi, d * kLog2eLo));
           }
         }
-        part = static_cast<double>(acc[0] + acc[1]) + static_cast<double>(acc[2] + acc[3]);
+        const double part = static_cast<double>((acc[0] + acc[1]) + (acc[2] + acc[3]));
+        const float higher = fmaxf(far, most);
+        far_sum = (far == -CUDART_INF_F ? 0.0 : far_sum * exp(static_cast<double>(far) - static_cast<double>(higher))) +
+                  part * exp(static_cast<double>(most) - static_cast<double>(higher));
+        far = higher;
+      } else if (anchor != -CUDART_INF_F) {
+        // exp(x) as 2^(x log2 e - anchor) with a whole anchor near the maximum: sums of
+        // different anchors differ by exact powers of two
+        const uint64_t hi = pack2(kLog2eHi, kLog2eHi), lo = pack2(kLog2eLo, kLog2eLo), back = pack2(-anchor, -anchor);
+        uint64_t acc[2] = {0, 0};
 #pragma unroll
-        for (int32_t d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(kFull, part, d);
-      }
-      if (top == -CUDART_INF_F) {
-        sum = part;
-        top = most;
-      } else {
-        const float higher = max_nan(top, most);
-        sum = sum * exp(static_cast<double>(top) - static_cast<double>(higher)) +
-              part * exp(static_cast<double>(most) - static_cast<double>(higher));
-        top = higher;
-      }
-    }
-    if (MASKED && !RENORMALIZE) {
+        for (int32_t j = 0; j < kVecs; ++j) {
+          if (kSkips && !__any_sync(kFull, (own >> (j * kPer)) & kAll)) continue;
 #pragma unroll
-      for (int32_t j = 0; j < kVecs; ++j)
-        if (bits[j] != (1u << kPer) - 1u) E::keep(v[j], bits[j]);
-      shown = E::top(v[0]);
-#pragma unroll
-      for (int32_t j = 1; j < kVecs; ++j) shown = max_nan(shown, E::top(v[j]));
-    }
-    // the bound, then every token that reaches it
-    uint32_t group = rising(shown + 0.0f);
-    for (int32_t d = 1; d < group_lanes; d <<= 1) group = max(group, __shfl_xor_sync(kFull, group, d));
-    if ((lane & (group_lanes - 1)) == 0) sh.group_top[tid / group_lanes] = group;
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    uint32_t bound = kFull;
-    for (int32_t g = lane; g < groups; g += 32) bound = min(bound, sh.group_top[g]);
-    bound = max(__reduce_min_sync(kFull, bound), bar);
-    const float reach = from_rising(bound);
-    if (shown >= reach) {
-#pragma unroll
-      for (int32_t j = 0; j < kVecs; ++j) {
-        if (!(E::top(v[j]) >= reach)) continue;
-        const int32_t t0 = (v0 + j * kScanThreads) * kPer - head;
-#pragma unroll
-        for (int32_t k = 0; k < kPer; ++k) {
-          const float x = E::at(v[j], k) + 0.0f;
-          if (x >= reach) {
-            const int32_t n = atomicAdd(&sh.count, 1);
-            if (n < kPushCap) sh.pushed[n] = make_key(rising(x), t0 + k);
+          for (int32_t k = 0; k < kPer; k += 2) {
+            const uint64_t x = pack2(E::at(v[j], k), E::at(v[j], k + 1));
+            const uint64_t y = fma2(x, lo, fma2(x, hi, back));
+            acc[(k >> 1) & 1] = add2(acc[(k >> 1) & 1], pack2(exp2_fast(low(y)), exp2_fast(high(y))));
           }
+        }
+        const uint64_t all = add2(acc[0], acc[1]);
+        sum += static_cast<double>(low(all) + high(all));
+      }
+      if (MASKED && !RENORMALIZE) {
+#pragma unroll
+        for (int32_t j = 0; j < kVecs; ++j) {
+          const uint32_t b = (own >> (j * kPer)) & kAll;
+          if (b != kAll) E::keep(v[j], b);
+        }
+        shown = E::top(v);
+      }
+      sh.tops[at][tid] = rising(shown + 0.0f);
+      best = fmaxf(best, shown);
+      // the slots are read: the step after the next
+      if (MASKED) {
+        bits[0] = bits[1];
+        bits[1] = own_bits(step + 2, word);
+        word = step + 3 < stop ? load_word(step + 3) : 0u;
+      }
+      if (step + 2 < stop) issue(step + 2, bits[1], slot);
+      commit_async();
+    }
+
+    // the best tokens of the round and of the keys held: the entries that reach the wanted-th of
+    // the threads' maxima (to its upper 16 bits) or, once enough are held, the last of them
+    const int32_t steps = stop - round;
+    const int32_t first = round * kStepTokens - head;
+    sh.thread_top[tid] = rising(best + 0.0f);
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    uint32_t bound = 0;
+    {
+      uint32_t of[kScanThreads / 32];
+#pragma unroll
+      for (int32_t i = 0; i < kScanThreads / 32; ++i) of[i] = sh.thread_top[i * 32 + lane];
+#pragma unroll 1
+      for (int32_t bit = 31; bit >= 16; --bit) {
+        const uint32_t trial = bound | (1u << bit);
+        int32_t reached = 0;
+#pragma unroll
+        for (int32_t i = 0; i < kScanThreads / 32; ++i) reached += of[i] >= trial;
+        if (__reduce_add_sync(kFull, reached) >= wanted) bound = trial;
+      }
+    }
+    bound = max(bound, kRisingLowest);
+    if (held == wanted) bound = max(bound, static_cast<uint32_t>(sh.few[wanted - 1] >> 32) + 1u);
+    for (int32_t at = 0; at < steps; ++at)
+      if (sh.tops[at][tid] >= bound) {
+        const int32_t n = atomicAdd(&sh.listed, 1);
+        if (n < kListCap) sh.list[n] = at * kScanThreads + tid;
+      }
+    __syncthreads();
+    if (sh.listed > kListCap) bound = max(bound, list_crowded(sh, steps, wanted));
+    const int32_t vectors = min(sh.listed, kListCap) * kVecs;
+    if (tid < held) sh.pushed[tid] = sh.few[tid];  // the table's memory: every entry has been read
+    if (tid == 0) sh.count = held;
+    __syncthreads();
+    const float least = from_rising(bound);
+    bool over = false;
+    for (int32_t i = tid; i < vectors; i += kScanThreads) {
+      const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
+      uint4 v = make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
+      if (t0 < vocab) {
+        v = load_vector<E>(logits, t0, vocab);
+        if (MASKED) E::keep(v, mask.bits(t0, kPer, vocab));
+      }
+      sh.ring[i] = v;
+#pragma unroll
+      for (int32_t k = 0; k < kPer; ++k) {
+        const float x = E::at(v, k) + 0.0f;
+        if (x >= least) {
+          const int32_t n = atomicAdd(&sh.count, 1);
+          if (n < kPushCap) sh.pushed[n] = make_key(rising(x), t0 + k);
+          over |= n >= kPushCap;
         }
       }
     }
-    __syncthreads();
-    int32_t pushed = sh.count;
-    if (pushed > kPushCap) {
-      // too many reach it (ties, or few allowed groups): the exact `wanted`-th best order
-      // number by bisection, then the token bound among its equals
-      uint32_t edge = 0;
-      int32_t turn = 0;
-      for (int32_t bit = 31; bit >= 0; --bit, turn ^= 1) {
-        const uint32_t trial = edge | (1u << bit);
-        int32_t mine = 0;
-#pragma unroll
-        for (int32_t j = 0; j < kVecs; ++j)
-#pragma unroll
-          for (int32_t k = 0; k < kPer; ++k) mine += rising(E::at(v[j], k) + 0.0f) >= trial;
-        if (block_total(mine, sh.counts[turn]) >= wanted) edge = trial;
-      }
-      int32_t above = 0;
-#pragma unroll
-      for (int32_t j = 0; j < kVecs; ++j)
-#pragma unroll
-        for (int32_t k = 0; k < kPer; ++k) above += rising(E::at(v[j], k) + 0.0f) > edge;
-      above = block_total(above, sh.counts[turn]);
-      turn ^= 1;
-      int32_t lowest = -1;  // equals up to lowest + 1 are taken
-      for (int32_t bit = 20; bit >= 0; --bit, turn ^= 1) {
-        const int32_t trial = lowest + (1 << bit);
-        int32_t mine = 0;
-#pragma unroll
-        for (int32_t j = 0; j < kVecs; ++j)
-#pragma unroll
-          for (int32_t k = 0; k < kPer; ++k)
-            mine += rising(E::at(v[j], k) + 0.0f) == edge && (v0 + j * kScanThreads) * kPer - head + k <= trial;
-        if (block_total(mine, sh.counts[turn]) < wanted - above) lowest = trial;
-      }
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-#pragma unroll
-      for (int32_t j = 0; j < kVecs; ++j) {
-        const int32_t t0 = (v0 + j * kScanThreads) * kPer - head;
-#pragma unroll
-        for (int32_t k = 0; k < kPer; ++k) {
-          const uint32_t o = rising(E::at(v[j], k) + 0.0f);
-          if (o > edge || (o == edge && t0 + k <= lowest + 1)) {
-            const int32_t n = atomicAdd(&sh.count, 1);
-            if (n < kPushCap) sh.pushed[n] = make_key(o, t0 + k);
-          }
-        }
-      }
-      __syncthreads();
-      pushed = min(sh.count, kPushCap);
-    }
-    // the best of those held and those pushed, in order, by counting the greater ones
-    const int32_t n = held + pushed;
-    const uint64_t* old = sh.best[which];
-    uint64_t* fresh = sh.best[which ^ 1];
-    for (int32_t i = tid; i < n; i += kScanThreads) {
-      const uint64_t mine = i < held ? old[i] : sh.pushed[i - held];
-      int32_t rank = 0;
-      for (int32_t j = 0; j < held; ++j) rank += old[j] > mine;
-      for (int32_t j = 0; j < pushed; ++j) rank += sh.pushed[j] > mine;
-      if (rank < wanted) fresh[rank] = mine;
-    }
-    __syncthreads();
-    which ^= 1;
-    held = min(n, wanted);
-    // a later token equal to the last of a full list comes after it
-    if (held == wanted) bar = max(bar, static_cast<uint32_t>(fresh[wanted - 1] >> 32) + 1u);
+    if (__syncthreads_or(over)) push_crowded<E>(sh, vectors, first, held, wanted);
+    held = best_of(sh, min(sh.count, kPushCap), wanted);
   }
-  if (lane == 0) {
-    sh.warp_top[warp] = top;
-    sh.warp_sum[warp] = sum;
+  if (!scans) return;  // a share past the row's end
+#pragma unroll
+  for (int32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+  if (far != -CUDART_INF_F) {  // uniform in the warp
+#pragma unroll
+    for (int32_t d = 16; d > 0; d >>= 1) far_sum += __shfl_xor_sync(kFull, far_sum, d);
   }
+  if (lane == 0) sh.warp_part[warp] = Part{sum, far_sum, anchor, far};
+  uint64_t* out = s.keys + static_cast<int64_t>(blockIdx.x) * wanted;
+  for (int32_t i = tid; i < wanted; i += kScanThreads) out[i] = i < held ? sh.few[i] : 0u;
   __syncthreads();
   if (warp == 0) {
-    const float t = lane < kScanWarps ? sh.warp_top[lane] : -CUDART_INF_F;
-    float most = t;
-#pragma unroll
-    for (int32_t d = 16; d > 0; d >>= 1) most = max_nan(most, __shfl_xor_sync(kFull, most, d));
-    double part = 0.0;
-    if (lane < kScanWarps && t != -CUDART_INF_F)
-      part = sh.warp_sum[lane] * exp(static_cast<double>(t) - static_cast<double>(most));
-#pragma unroll
-    for (int32_t d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(kFull, part, d);
-    if (lane == 0) s.parts[blockIdx.x] = Part{part, most, 0};
+    Part p = lane < kScanWarps ? sh.warp_part[lane] : Part{0.0, 0.0, -CUDART_INF_F, -CUDART_INF_F};
+    p = total_part(p);
+    if (lane == 0) s.parts[blockIdx.x] = p;
   }
-  uint64_t* out = s.keys + static_cast<int64_t>(blockIdx.x) * wanted;
-  for (int32_t i = tid; i < wanted; i += kScanThreads) out[i] = i < held ? sh.best[which][i] : 0u;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -446,31 +708,33 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_kernel(const __grid_cons
 constexpr int32_t kMergeThreads = 512;
 constexpr int32_t kMergeWarps = kMergeThreads / 32;
 constexpr int32_t kSamples = 1024;
+constexpr double kLn2 = 0.693147180559945309417;
 // Two beams' candidates nearer than this are ordered by log-sums taken again in 64 bits.
 constexpr double kNear = 1e-6;
 
 struct MergeShared {
   double sample[kSamples];
-  double log_sum[kMaxBeams];
+  double log_sum[kMaxBeams];   // log of the row's sum of exp(x - ref)
+  double ref[kMaxBeams];
   double score[kMaxBeams];
-  float top[kMaxBeams];
-  int32_t state[kMaxBeams];   // 0 offers nothing, 1 candidates, 2 ended, 3 candidates, 64-bit sum
+  int32_t state[kMaxBeams];    // 0 offers nothing, 1 candidates, 2 ended, 3 candidates, 64-bit sum
   int32_t again[kMaxBeams];
-  int32_t order[kMaxCandidates + 1];
+  double best[kMaxCandidates];
+  uint32_t best_code[kMaxCandidates];
   double warp_sum[kMergeWarps];
   double bound;
   int32_t count, near;
 };
 
-// Sum over N_r of exp(x - top) in 64 bits, by the whole CTA.
+// Sum over N_r of exp(x - ref) in 64 bits, by the whole CTA.
 template <typename E>
-__device__ double row_sum(const SelectArgs& a, int32_t row, float top, double (&scratch)[kMergeWarps]) {
+__device__ double row_sum(const SelectArgs& a, int32_t row, double ref, double (&scratch)[kMergeWarps]) {
   const char* logits = a.logits + static_cast<int64_t>(row) * a.row_stride * E::kBytes;
   const RowMask mask = a.renormalize ? row_mask(a.masks, row) : RowMask{nullptr, nullptr};
   double sum = 0.0;
   for (int32_t t = threadIdx.x; t < a.vocab; t += kMergeThreads) {
     if (!mask.all() && !((mask.word(t >> 5) >> (t & 31)) & 1u)) continue;
-    sum += exp(static_cast<double>(E::one(logits + static_cast<int64_t>(t) * E::kBytes)) - static_cast<double>(top));
+    sum += exp(static_cast<double>(E::one(logits + static_cast<int64_t>(t) * E::kBytes)) - ref);
   }
 #pragma unroll
   for (int32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
@@ -482,6 +746,13 @@ __device__ double row_sum(const SelectArgs& a, int32_t row, float top, double (&
   return sum;
 }
 
+// How many threads of a warp share one item's comparisons with n others.
+__device__ __forceinline__ int32_t split_of(int32_t n) {
+  int32_t split = 1;
+  while (split < 32 && n * split * 2 <= kMergeThreads) split <<= 1;
+  return split;
+}
+
 template <typename E>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ ScanArgs s) {
   extern __shared__ __align__(16) char dynamic[];
@@ -489,8 +760,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   const SelectArgs& a = s.a;
   const int32_t pool = s.pool, beams = a.beams, shares = s.shares, wanted = a.candidates;
   double* value = reinterpret_cast<double*>(dynamic);            // [pool]; -inf: none
-  uint32_t* code = reinterpret_cast<uint32_t*>(value + pool);    // [pool] beam << 20 | token
-  int32_t* kept = reinterpret_cast<int32_t*>(code + pool);       // [pool] places above the bound
+  double* kept = value + pool;                                   // [pool] values above the bound,
+  uint32_t* code = reinterpret_cast<uint32_t*>(kept + pool);     // [pool] beam << 20 | token
+  uint32_t* kept_code = code + pool;                             // [pool]
   const int32_t group = blockIdx.x, row0 = group * beams;
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the scan is complete
@@ -499,29 +771,46 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     const int32_t row = row0 + b;
     const float score = a.scores[row];
     int32_t state = 0;
-    float top = -CUDART_INF_F;
-    double sum = 0.0;
+    double ref = 0.0, log_sum = 0.0;
     if (isfinite(score)) {
       if (a.finished && a.finished[row]) {
         state = 2;
       } else {
-        for (int32_t c = lane; c < shares; c += 32) top = max_nan(top, s.parts[row * shares + c].top);
-#pragma unroll
-        for (int32_t d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, d));
-        for (int32_t c = lane; c < shares; c += 32) {
-          const Part p = s.parts[row * shares + c];
-          if (p.top != -CUDART_INF_F) sum += p.sum * exp(static_cast<double>(p.top) - static_cast<double>(top));
+        Part p{0.0, 0.0, -CUDART_INF_F, -CUDART_INF_F};
+        for (int32_t c = lane; c < shares; c += 32) {  // at most a few for a lane
+          const Part q = s.parts[static_cast<int64_t>(row) * shares + c];
+          if (q.anchor != -CUDART_INF_F) {
+            const float anchor = fmaxf(p.anchor, q.anchor);
+            p.sum = (p.anchor == -CUDART_INF_F ? 0.0 : p.sum * power2(p.anchor - anchor)) + q.sum * power2(q.anchor - anchor);
+            p.anchor = anchor;
+          }
+          if (q.far != -CUDART_INF_F) {
+            const float far = fmaxf(p.far, q.far);
+            p.far_sum = (p.far == -CUDART_INF_F ? 0.0 : p.far_sum * exp(static_cast<double>(p.far) - static_cast<double>(far))) +
+                        q.far_sum * exp(static_cast<double>(q.far) - static_cast<double>(far));
+            p.far = far;
+          }
         }
-#pragma unroll
-        for (int32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-        state = isfinite(sum) && sum > 0.0 ? 1 : 0;
+        p = total_part(p);
+        double sum = p.sum;
+        ref = p.anchor == -CUDART_INF_F ? 0.0 : static_cast<double>(p.anchor) * kLn2;
+        if (p.far != -CUDART_INF_F) {
+          const double far = static_cast<double>(p.far);
+          const double higher = p.anchor == -CUDART_INF_F || far > ref ? far : ref;
+          sum = (p.anchor == -CUDART_INF_F ? 0.0 : sum * exp(ref - higher)) + p.far_sum * exp(far - higher);
+          ref = higher;
+        }
+        if (isfinite(sum) && sum > 0.0) {
+          state = 1;
+          log_sum = log(sum);
+        }
       }
     }
     if (lane == 0) {
       sh.score[b] = score;
       sh.state[b] = state;
-      sh.top[b] = top;
-      sh.log_sum[b] = state == 1 ? log(sum) : 0.0;
+      sh.ref[b] = ref;
+      sh.log_sum[b] = log_sum;
     }
   }
   const int32_t lists = beams * shares;
@@ -542,14 +831,18 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         if (key) {
           token = static_cast<int32_t>(~static_cast<uint32_t>(key));
           const float x = from_rising(static_cast<uint32_t>(key >> 32));
-          v = sh.score[b] + ((static_cast<double>(x) - static_cast<double>(sh.top[b])) - sh.log_sum[b]);
+          v = sh.score[b] + ((static_cast<double>(x) - sh.ref[b]) - sh.log_sum[b]);
           if (!isfinite(__double2float_rn(v))) v = -CUDART_INF;
         }
       }
       value[i] = v;
       code[i] = (static_cast<uint32_t>(b) << 20) | static_cast<uint32_t>(token);
     }
-    if (tid == 0) sh.count = sh.near = 0;
+    for (int32_t b = tid; b < beams; b += kMergeThreads) sh.again[b] = 0;
+    if (tid == 0) {
+      sh.count = sh.near = 0;
+      sh.bound = -CUDART_INF;
+    }
     __syncthreads();
     // a bound that `wanted` candidates reach: the wanted-th best of a sample of distinct ones,
     // the lists' first places (their maxima over 4 * wanted sets of lists, if there are more)
@@ -564,54 +857,86 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
     } else {
       const int32_t places = min((target + lists - 1) / lists, wanted);
-      samples = lists * places;  // at most target + lists <= 8 * wanted <= kSamples
+      samples = lists * places;  // fewer than target + lists < 8 * wanted <= kSamples
       for (int32_t i = tid; i < samples; i += kMergeThreads) {
         const int32_t l = i / places;
         sh.sample[i] = value[l * wanted + (i - l * places)];
       }
     }
-    if (tid == 0) sh.bound = -CUDART_INF;
     __syncthreads();
-    for (int32_t i = tid; i < samples; i += kMergeThreads) {
-      const double mine = sh.sample[i];
-      int32_t rank = 0;
-      for (int32_t j = 0; j < samples; ++j) rank += sh.sample[j] > mine || (sh.sample[j] == mine && j < i);
-      if (rank == wanted - 1) sh.bound = mine;
+    {
+      const int32_t split = split_of(samples), step = kMergeThreads / split, part = tid & (split - 1);
+      for (int32_t i0 = 0; i0 < samples; i0 += step) {  // uniform: the shuffles below take whole warps
+        const int32_t i = i0 + tid / split;
+        int32_t rank = 0;
+        const double mine = i < samples ? sh.sample[i] : 0.0;
+        if (i < samples)
+          for (int32_t j = part; j < samples; j += split) {
+            const double other = sh.sample[j];
+            rank += other > mine || (other == mine && j < i);
+          }
+        for (int32_t d = 1; d < split; d <<= 1) rank += __shfl_xor_sync(kFull, rank, d);
+        if (i < samples && part == 0 && rank == wanted - 1) sh.bound = mine;
+      }
     }
     __syncthreads();
     const double bound = sh.bound - 2.0 * kNear;
     for (int32_t i = tid; i < pool; i += kMergeThreads)
-      if (value[i] > -CUDART_INF && value[i] >= bound) kept[atomicAdd(&sh.count, 1)] = i;
+      if (value[i] > -CUDART_INF && value[i] >= bound) {
+        const int32_t at = atomicAdd(&sh.count, 1);
+        kept[at] = value[i];
+        kept_code[at] = code[i];
+      }
     __syncthreads();
     const int32_t n = sh.count;
-    for (int32_t i = tid; i < n; i += kMergeThreads) {
-      const int32_t at = kept[i];
-      const double mine = value[at];
-      const uint32_t own = code[at];
-      int32_t rank = 0;
-      for (int32_t j = 0; j < n; ++j) {
-        const double other = value[kept[j]];
-        rank += other > mine || (other == mine && code[kept[j]] < own);
+    {
+      const int32_t split = split_of(n), step = kMergeThreads / split, part = tid & (split - 1);
+      for (int32_t i0 = 0; i0 < n; i0 += step) {
+        const int32_t i = i0 + tid / split;
+        int32_t rank = 0;  // and, from bit 16 on, how many of other beams are too near to tell
+        const double mine = i < n ? kept[i] : 0.0;
+        const uint32_t own = i < n ? kept_code[i] : 0u;
+        if (i < n)
+          for (int32_t j = part; j < n; j += split) {
+            const double ahead = kept[j] - mine;
+            const uint32_t other = kept_code[j];
+            rank += ahead > 0.0 || (ahead == 0.0 && other < own);
+            rank += fabs(ahead) <= kNear && ((other ^ own) >> 20) ? 1 << 16 : 0;
+          }
+        for (int32_t d = 1; d < split; d <<= 1) rank += __shfl_xor_sync(kFull, rank, d);
+        if (i < n && part == 0) {
+          if (rank >> 16) sh.near = 1;
+          rank &= 0xffff;
+          if (rank < wanted) {
+            sh.best[rank] = mine;
+            sh.best_code[rank] = own;
+          }
+        }
       }
-      if (rank <= wanted) sh.order[rank] = at;
     }
-    for (int32_t b = tid; b < beams; b += kMergeThreads) sh.again[b] = 0;
     __syncthreads();
-    // neighbours of different beams whose order the 32-bit sums cannot tell
-    const int32_t listed = min(n, wanted + 1);
-    for (int32_t i = tid; i + 1 < listed; i += kMergeThreads) {
-      const int32_t p = sh.order[i], q = sh.order[i + 1];
-      const int32_t bp = code[p] >> 20, bq = code[q] >> 20;
-      if (bp != bq && value[p] - value[q] <= kNear) {
-        if (sh.state[bp] == 1) sh.again[bp] = sh.near = 1;
-        if (sh.state[bq] == 1) sh.again[bq] = sh.near = 1;
-      }
+    if (!sh.near) break;
+    // beams with a candidate that may belong among the best and whose order against another
+    // beam's the 32-bit sums cannot tell
+    const double least = n > wanted ? sh.best[wanted - 1] - kNear : -CUDART_INF;
+    __syncthreads();
+    if (tid == 0) sh.near = 0;
+    __syncthreads();
+    for (int32_t i = tid; i < n; i += kMergeThreads) {
+      const double mine = kept[i];
+      const int32_t own = kept_code[i] >> 20;
+      if (mine < least || sh.state[own] != 1) continue;
+      for (int32_t j = 0; j < n; ++j)
+        if (fabs(kept[j] - mine) <= kNear && static_cast<int32_t>(kept_code[j] >> 20) != own) {
+          sh.again[own] = sh.near = 1;
+          break;
+        }
     }
     __syncthreads();
     if (!sh.near) break;
     for (int32_t b = 0; b < beams; ++b) {  // at most once for each beam
       if (!sh.again[b]) continue;
-      const double sum = row_sum<E>(a, row0 + b, sh.top[b], sh.warp_sum);
+      const double sum = row_sum<E>(a, row0 + b, sh.ref[b], sh.warp_sum);
       if (tid == 0) {
         sh.log_sum[b] = log(sum);
         sh.state[b] = 3;
@@ -623,11 +948,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     float score = -CUDART_INF_F;
     int32_t beam = -1, token = -1;
     bool ended = false;
-    if (i < sh.count) {
-      const int32_t at = sh.order[i];
-      score = __double2float_rn(value[at]);
-      beam = static_cast<int32_t>(code[at] >> 20);
-      token = static_cast<int32_t>(code[at] & 0xfffffu);
+    if (i < min(sh.count, wanted)) {
+      score = __double2float_rn(sh.best[i]);
+      beam = static_cast<int32_t>(sh.best_code[i] >> 20);
+      token = static_cast<int32_t>(sh.best_code[i] & 0xfffffu);
       ended = token == a.end_token || sh.state[beam] == 2;
     }
     a.out_scores[to] = score;
@@ -900,10 +1224,10 @@ int plan(int32_t groups, int32_t beams, int32_t vocab, int32_t dtype, int32_t ca
   int32_t sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int32_t per = dtype == XG_F32 ? 4 : 8;
-  // a misaligned row's vectors may start a vector early
-  const int32_t tiles = (vocab + 2 * per - 1) / per / (kScanThreads * kVecs) + 1;
+  const int32_t step = kScanThreads * kVecs * per;  // a misaligned row's vectors start up to a vector early
+  const int32_t tiles = (vocab + per - 1 + step - 1) / step;
   const int64_t rows = static_cast<int64_t>(groups) * beams;
-  int64_t shares = rows > 0 ? (static_cast<int64_t>(sms) * 8 + rows - 1) / rows : 1;
+  int64_t shares = rows > 0 ? (static_cast<int64_t>(sms) * 4 + rows - 1) / rows : 1;
   if (shares > kPoolMax / (beams * candidates)) shares = kPoolMax / (beams * candidates);
   if (shares > tiles) shares = tiles;
   if (shares < 1) shares = 1;
@@ -919,19 +1243,18 @@ int launch_select(const ScanArgs& s, cudaStream_t stream) {
   const SelectArgs& a = s.a;
   const bool masked = a.masks.words || a.masks.slots;
   const unsigned grid = static_cast<unsigned>(a.groups) * a.beams * s.shares;
-  if (!masked)
-    scan_kernel<E, false, true><<<grid, kScanThreads, 0, stream>>>(s);
-  else if (a.renormalize)
-    scan_kernel<E, true, true><<<grid, kScanThreads, 0, stream>>>(s);
-  else
-    scan_kernel<E, true, false><<<grid, kScanThreads, 0, stream>>>(s);
+  static std::atomic<bool> allowed_scan[3][kDevices], allowed[kDevices];
+  const auto scan = !masked ? scan_kernel<E, false, true> : a.renormalize ? scan_kernel<E, true, true> : scan_kernel<E, true, false>;
+  if (int rc = allow_shared(reinterpret_cast<const void*>(scan), sizeof(ScanShared),
+                            allowed_scan[!masked ? 0 : a.renormalize ? 1 : 2]))
+    return rc;
+  scan<<<grid, kScanThreads, sizeof(ScanShared), stream>>>(s);
   XG_BEAM_CUDA(cudaGetLastError(), "beam scan kernel");
-  static std::atomic<bool> allowed[kDevices];
-  if (int rc = allow_shared(reinterpret_cast<const void*>(merge_kernel<E>), kPoolMax * 16, allowed)) return rc;
+  if (int rc = allow_shared(reinterpret_cast<const void*>(merge_kernel<E>), kPoolMax * 24, allowed)) return rc;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.groups));
   config.blockDim = dim3(kMergeThreads);
-  config.dynamicSmemBytes = static_cast<size_t>(s.pool) * 16;
+  config.dynamicSmemBytes = static_cast<size_t>(s.pool) * 24;
   config.stream = stream;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the scan's end
