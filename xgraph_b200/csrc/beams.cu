@@ -964,11 +964,15 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
 // ---------------------------------------------------------------------------------------
 // Reordering.
 //
-// A thread owns one unit (up to 16 bytes) of every row of a group: it loads the unit from
-// each moved row's parent, then stores them, so the move is in place without a copy of the
-// rows, whatever cycles the parents form, and each byte that stays is not touched.
+// A thread owns a unit (up to 16 bytes) of every row of a group: it brings the unit of each row
+// that is someone's parent into its own slots in shared memory (cp.async), waits for them, then
+// stores each moved row's from its parent's slot.  So the move is in place whatever cycles the
+// parents form, a parent is read once however many children it has, and rows that stay are not
+// touched.  A thread fills its slots with as many units as they hold at a time; the CTAs of an
+// SM overlap one's loads with another's stores.
 
-constexpr int32_t kMoveThreads = 256;
+constexpr int32_t kMoveThreads = 128;
+constexpr int32_t kMoveSlots = 24;    // 16-byte slots of a thread (or one per beam, if more)
 constexpr int32_t kMoveTensors = 64;  // descriptors of one launch
 
 struct MoveTensor {
@@ -983,102 +987,185 @@ struct MoveTensor {
 
 struct MoveArgs {
   MoveTensor tensors[kMoveTensors];
-  int32_t count, groups, beams;
+  int32_t count, groups, beams, slots;
   int64_t rows;
   const int32_t* parents;
   const int32_t* lengths;
   const int32_t* row_of;
 };
 
-template <int32_t MOST, typename V>
-__device__ __forceinline__ void move_unit(const MoveTensor& t, int64_t offset, int32_t moved, const int32_t* from,
-                                          const int32_t* to) {
-  V held[MOST];
-  char* at = t.data + offset;
-#pragma unroll
-  for (int32_t i = 0; i < MOST; ++i)
-    if (i < moved) held[i] = *reinterpret_cast<const V*>(at + from[i] * t.row_bytes);
-#pragma unroll
-  for (int32_t i = 0; i < MOST; ++i)
-    if (i < moved) *reinterpret_cast<V*>(at + to[i] * t.row_bytes) = held[i];
+// One unit of 1 << LOG bytes into a slot, and out of it.
+template <int32_t LOG>
+__device__ __forceinline__ void fetch_unit(char* slot, const char* from) {
+  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
+  if constexpr (LOG == 4)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else if constexpr (LOG == 3)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+  else if constexpr (LOG == 2)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+  else if constexpr (LOG == 1)
+    *reinterpret_cast<uint16_t*>(slot) = *reinterpret_cast<const uint16_t*>(from);
+  else
+    *slot = *from;
+}
+template <int32_t LOG>
+__device__ __forceinline__ void store_unit(char* to, const char* slot) {
+  if constexpr (LOG == 4)
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(slot);
+  else if constexpr (LOG == 3)
+    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(slot);
+  else if constexpr (LOG == 2)
+    *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(slot);
+  else if constexpr (LOG == 1)
+    *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(slot);
+  else
+    *to = *slot;
 }
 
-template <int32_t MOST>
+// A group's moves: rows to read, and rows to write with the slot that each is written from.
+struct Moves {
+  int32_t source_row[kMaxBeams], target_row[kMaxBeams], target_slot[kMaxBeams];
+  unsigned long long parents;
+  int32_t sources, targets;
+};
+
+// The CTA's tiles of one tensor: every gridDim.x-th.
+// Long runs: a tile is a stretch of one run, so that a thread's units follow at fixed distances.
+// Short ones: a thread's units are found one by one among all runs' units.
+template <int32_t LOG>
+__device__ __forceinline__ void move_tensor(const MoveTensor& t, uint32_t size1, uint32_t size2, uint32_t size3,
+                                            const Moves& m, char* slots, int32_t slot_count) {
+  constexpr int32_t kSlot = kMoveThreads * 16;  // bytes from slot to slot
+  constexpr int32_t kNext = kMoveThreads << LOG;
+  const int32_t sources = m.sources, targets = m.targets;
+  const uint32_t batch = slot_count / sources;  // units a thread holds at a time
+  const uint32_t tile_units = batch * kMoveThreads;
+  const uint32_t runs = size1 * size2;
+  char* mine = slots + threadIdx.x * 16;
+  if (runs == 1 || size3 >= tile_units) {
+    const uint32_t of_run = (size3 + tile_units - 1) / tile_units;
+    const uint64_t tiles = static_cast<uint64_t>(runs) * of_run;
+    for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+      const uint32_t run = runs == 1 ? 0u : static_cast<uint32_t>(tile) / of_run;
+      const uint32_t unit = static_cast<uint32_t>(tile - static_cast<uint64_t>(run) * of_run) * tile_units + threadIdx.x;
+      const int32_t n = unit >= size3 ? 0 : static_cast<int32_t>(min(batch, (size3 - unit + kMoveThreads - 1) / kMoveThreads));
+      const uint32_t i1 = run / size2, i2 = run - i1 * size2;
+      char* at = t.data + (i1 * t.stride1 + i2 * t.stride2 + (static_cast<int64_t>(unit) << LOG));
+      for (int32_t i = 0; i < sources; ++i) {
+        const char* from = at + m.source_row[i] * t.row_bytes;
+        char* slot = mine + i * kSlot;
+#pragma unroll 4
+        for (int32_t u = 0; u < n; ++u, from += kNext, slot += sources * kSlot) fetch_unit<LOG>(slot, from);
+      }
+      commit_async();
+      wait_async<0>();
+      for (int32_t i = 0; i < targets; ++i) {
+        char* to = at + m.target_row[i] * t.row_bytes;
+        const char* slot = mine + m.target_slot[i] * kSlot;
+#pragma unroll 4
+        for (int32_t u = 0; u < n; ++u, to += kNext, slot += sources * kSlot) store_unit<LOG>(to, slot);
+      }
+    }
+  } else {
+    const uint64_t units = static_cast<uint64_t>(runs) * size3;
+    const uint64_t tiles = (units + tile_units - 1) / tile_units;
+    const auto place = [&](uint64_t unit) {
+      const uint32_t run = units <= 0xffffffffu ? static_cast<uint32_t>(unit) / size3 : static_cast<uint32_t>(unit / size3);
+      const uint32_t in_run = static_cast<uint32_t>(unit - static_cast<uint64_t>(run) * size3);
+      const uint32_t i1 = run / size2, i2 = run - i1 * size2;
+      return t.data + (i1 * t.stride1 + i2 * t.stride2 + (static_cast<int64_t>(in_run) << LOG));
+    };
+    for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+      const uint64_t unit0 = tile * tile_units + threadIdx.x;
+      char* slot = mine;
+      for (uint32_t u = 0; u < batch && unit0 + u * kMoveThreads < units; ++u) {
+        const char* at = place(unit0 + u * kMoveThreads);
+        for (int32_t i = 0; i < sources; ++i, slot += kSlot) fetch_unit<LOG>(slot, at + m.source_row[i] * t.row_bytes);
+      }
+      commit_async();
+      wait_async<0>();
+      slot = mine;
+      for (uint32_t u = 0; u < batch && unit0 + u * kMoveThreads < units; ++u, slot += sources * kSlot) {
+        char* at = place(unit0 + u * kMoveThreads);
+        for (int32_t i = 0; i < targets; ++i)
+          store_unit<LOG>(at + m.target_row[i] * t.row_bytes, slot + m.target_slot[i] * kSlot);
+      }
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveArgs a) {
-  __shared__ int32_t from[kMaxBeams], to[kMaxBeams];
-  __shared__ int32_t moves;
-  const int32_t group = blockIdx.y;
-  if (threadIdx.x < 32) {
-    int32_t n = 0;
-    for (int32_t b0 = 0; b0 < a.beams; b0 += 32) {
-      const int32_t b = b0 + static_cast<int32_t>(threadIdx.x);
-      int32_t source = -1, target = -1;
+  extern __shared__ __align__(16) char slots[];  // [slot][thread] of 16 bytes
+  __shared__ Moves m;
+  const int32_t group = blockIdx.y, tid = threadIdx.x;
+  if (tid < 32) {
+    if (tid == 0) m.parents = 0;
+    __syncwarp();
+    int32_t n = 0, parent[2], target[2], source[2];
+    uint32_t who[2];
+#pragma unroll
+    for (int32_t h = 0; h < 2; ++h) {
+      const int32_t b = tid + 32 * h;
+      parent[h] = source[h] = target[h] = -1;
       if (b < a.beams) {
-        const int32_t parent = a.parents[group * a.beams + b];
-        if (parent >= 0 && parent < a.beams && parent != b) {
-          source = group * a.beams + parent;
-          target = group * a.beams + b;
+        parent[h] = a.parents[group * a.beams + b];
+        if (parent[h] >= 0 && parent[h] < a.beams && parent[h] != b) {
+          source[h] = group * a.beams + parent[h];
+          target[h] = group * a.beams + b;
           if (a.row_of) {
-            source = a.row_of[source];
-            target = a.row_of[target];
+            source[h] = a.row_of[source[h]];
+            target[h] = a.row_of[target[h]];
           }
         }
       }
-      const bool valid = source >= 0 && source < a.rows && target >= 0 && target < a.rows && source != target;
-      const uint32_t who = __ballot_sync(kFull, valid);
-      if (valid) {
-        const int32_t at = n + __popc(who & ((1u << threadIdx.x) - 1u));
-        from[at] = source;
-        to[at] = target;
-      }
-      n += __popc(who);
+      const bool valid = source[h] >= 0 && source[h] < a.rows && target[h] >= 0 && target[h] < a.rows && source[h] != target[h];
+      who[h] = __ballot_sync(kFull, valid);
+      if (valid) atomicOr(&m.parents, 1ull << parent[h]);
     }
-    if (threadIdx.x == 0) moves = n;
+    __syncwarp();
+    const unsigned long long used = m.parents;
+#pragma unroll
+    for (int32_t h = 0; h < 2; ++h) {
+      if ((who[h] >> tid) & 1u) {
+        const int32_t at = n + __popc(who[h] & ((1u << tid) - 1u));
+        const int32_t slot = __popcll(used & ((1ull << parent[h]) - 1ull));
+        m.target_row[at] = target[h];
+        m.target_slot[at] = slot;
+        m.source_row[slot] = source[h];  // the same from every child of the parent
+      }
+      n += __popc(who[h]);
+    }
+    if (tid == 0) {
+      m.targets = n;
+      m.sources = __popcll(used);
+    }
   }
+  const uint32_t length = a.lengths ? static_cast<uint32_t>(max(a.lengths[group], 0)) : 0x7fffffffu;
   __syncthreads();
-  const int32_t moved = moves;
-  if (moved == 0) return;
-  const int32_t length = a.lengths ? max(a.lengths[group], 0) : 0x7fffffff;
-  uint64_t next = blockIdx.x, first = 0;
-  for (int32_t k = 0; k < a.count; ++k) {
-    const MoveTensor& t = a.tensors[k];
-    const uint32_t size1 = t.axis == 1 ? min(t.size1, static_cast<uint32_t>(length)) : t.size1;
-    const uint32_t size2 = t.axis == 2 ? min(t.size2, static_cast<uint32_t>(length)) : t.size2;
-    const uint32_t size3 =
-        t.axis == 3 ? static_cast<uint32_t>(min(static_cast<uint64_t>(t.size3), static_cast<uint64_t>(t.unit) * length))
-                    : t.size3;
-    const uint64_t units = t.axis == 4 && length == 0 ? 0 : static_cast<uint64_t>(size1) * size2 * size3;
-    const uint64_t tiles = (units + kMoveThreads - 1) / kMoveThreads;
-    for (; next < first + tiles; next += gridDim.x) {
-      const uint64_t unit = (next - first) * kMoveThreads + threadIdx.x;
-      if (unit >= units) continue;
-      int64_t offset;
-      if (size3 == units) {
-        offset = static_cast<int64_t>(unit) << t.log_bytes;
-      } else {
-        const uint64_t outer = unit / size3;
-        const uint32_t i1 = static_cast<uint32_t>(outer / size2), i2 = static_cast<uint32_t>(outer - static_cast<uint64_t>(i1) * size2);
-        offset = i1 * t.stride1 + i2 * t.stride2 + (static_cast<int64_t>(unit - outer * size3) << t.log_bytes);
-      }
-      switch (t.log_bytes) {
-        case 4:
-          if constexpr (MOST <= 32) move_unit<MOST, uint4>(t, offset, moved, from, to);
-          break;
-        case 3: move_unit<MOST, uint2>(t, offset, moved, from, to); break;
-        case 2: move_unit<MOST, uint32_t>(t, offset, moved, from, to); break;
-        case 1: move_unit<MOST, uint16_t>(t, offset, moved, from, to); break;
-        default: move_unit<MOST, uint8_t>(t, offset, moved, from, to); break;
-      }
-    }
-    first += tiles;
+  if (m.targets == 0) return;
+  const MoveTensor& t = a.tensors[blockIdx.z];
+  const uint32_t size1 = t.axis == 1 ? min(t.size1, length) : t.size1;
+  const uint32_t size2 = t.axis == 2 ? min(t.size2, length) : t.size2;
+  const uint32_t size3 =
+      t.axis == 3 ? static_cast<uint32_t>(min(static_cast<uint64_t>(t.size3), static_cast<uint64_t>(t.unit) * length))
+                  : t.size3;
+  if (size1 == 0 || size2 == 0 || size3 == 0 || (t.axis == 4 && length == 0)) return;
+  switch (t.log_bytes) {
+    case 4: move_tensor<4>(t, size1, size2, size3, m, slots, a.slots); break;
+    case 3: move_tensor<3>(t, size1, size2, size3, m, slots, a.slots); break;
+    case 2: move_tensor<2>(t, size1, size2, size3, m, slots, a.slots); break;
+    case 1: move_tensor<1>(t, size1, size2, size3, m, slots, a.slots); break;
+    default: move_tensor<0>(t, size1, size2, size3, m, slots, a.slots); break;
   }
 }
 
 // ---------------------------------------------------------------------------------------
 // The back-trace.
 
-constexpr int32_t kTraceThreads = 512;
-constexpr int32_t kTraceBytes = 96 * 1024;  // shared memory for a window's parents
+constexpr int32_t kTraceThreads = 256;
+constexpr int32_t kTraceWarps = kTraceThreads / 32;
+constexpr int32_t kTraceBytes = 96 * 1024;  // shared memory for a window
 constexpr uint8_t kNoBeam = 0xff;
 
 struct TraceArgs {
@@ -1088,73 +1175,118 @@ struct TraceArgs {
   int64_t parent_step, parent_group;
   int32_t steps, groups, beams;
   const int32_t* lengths;
-  int32_t pad, window, segment;
+  int32_t pad, window, way_stride, segment, segments, cluster, log_lanes;
   int32_t* out;
 };
 
-// One CTA per group, windows of steps from the last to the first.  A window's parent maps sit
-// in shared memory as bytes; its segments are walked in parallel twice: once from every
-// beam, which gives each segment's map, and, after the maps are chained, once more along the
-// beams that each last place came through, which leaves every step's beam in shared memory
-// for the tokens' gather.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint8_t peer_byte(const uint8_t* mine, int32_t rank) {
+  uint32_t at, got;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(at)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+  asm volatile("ld.shared::cluster.u8 %0, [%1];" : "=r"(got) : "r"(at) : "memory");
+  return static_cast<uint8_t>(got);
+}
+
+// Four bytes, asynchronously.
+__device__ __forceinline__ void copy_word_async(void* shared, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared))),
+               "l"(global)
+               : "memory");
+}
+
+// A cluster of CTAs per group takes stretches of cluster * window steps, from the last to the
+// first; each CTA one window.  A window's tokens and parent maps (as bytes) sit in its shared
+// memory, cut into segments that threads walk in parallel from every beam.  The segments' maps
+// chained give the window's, the later windows' maps (read from the cluster's other CTAs) the
+// beam at the window's end of each last place, and a second walk of the segments every step's
+// beam, by which the tokens are picked.  So the walk is 2 * segment + segments + cluster links
+// long instead of the steps', and the rest is loads and stores side by side.
 __global__ void __launch_bounds__(kTraceThreads) trace_kernel(const __grid_constant__ TraceArgs a) {
-  extern __shared__ __align__(16) uint8_t maps[];  // [window][beams], then [window][beams] ways, then segments' maps
-  const int32_t group = blockIdx.x, beams = a.beams, tid = threadIdx.x;
+  extern __shared__ __align__(16) uint8_t shared[];
+  const int32_t beams = a.beams, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t* text = reinterpret_cast<int32_t*>(shared);        // [window][beams + 1]: rows shifted by a bank each
+  uint8_t* maps = shared + a.window * (beams + 1) * 4;       // [window][beams]
+  uint8_t* way = maps + a.window * beams;                    // [beams][way_stride]: the beam of each last place
+  uint8_t* through = way + beams * a.way_stride;             // [segments][beams]: from a segment's end to before it
+  uint8_t* enter = through + a.segments * beams;             // [segments][beams]: the beam at its end, per last place
+  uint8_t* whole = enter + a.segments * beams;               // [beams]: from the window's end to before it
+  uint8_t* carry = whole + kMaxBeams;                        // [beams]: the beam at the stretch's end, per last place
+  const int32_t group = blockIdx.x / a.cluster, rank = blockIdx.x - group * a.cluster;
   const int32_t length = a.lengths ? min(max(a.lengths[group], 0), a.steps) : a.steps;
-  uint8_t* way = maps + a.window * beams;
-  const int32_t segments_most = (a.window + a.segment - 1) / a.segment;
-  uint8_t* through = way + a.window * beams;              // [segments][beams]: from the segment's end to before it
-  uint8_t* enter = through + segments_most * beams;       // [segments][beams]: the beam at the segment's end, per last place
-  uint8_t* carry = enter + segments_most * beams;         // [beams]: the beam at the window's end, per last place
   int32_t* out = a.out + static_cast<int64_t>(group) * beams * a.steps;
-  for (int64_t i = tid; i < static_cast<int64_t>(beams) * (a.steps - length); i += kTraceThreads) {
-    const int32_t k = static_cast<int32_t>(i / (a.steps - length));
-    out[static_cast<int64_t>(k) * a.steps + length + (i - static_cast<int64_t>(k) * (a.steps - length))] = a.pad;
-  }
+  // threads by beam: 1 << log_lanes >= beams of them to a step or a segment
+  const int32_t k_own = tid & ((1 << a.log_lanes) - 1), s_own = tid >> a.log_lanes, s_next = kTraceThreads >> a.log_lanes;
+  const bool has_beam = k_own < beams;
   for (int32_t k = tid; k < beams; k += kTraceThreads) carry[k] = static_cast<uint8_t>(k);
-  for (int32_t end = length; end > 0; end -= a.window) {
-    const int32_t begin = max(0, end - a.window), count = end - begin;
+  const int32_t stretch = a.window * a.cluster;
+  for (int32_t stop = length; stop > 0; stop -= stretch) {
+    // rank 0 the last window of the stretch
+    const int32_t end = max(stop - rank * a.window, 0), begin = max(end - a.window, 0), count = end - begin;
     const int32_t segments = (count + a.segment - 1) / a.segment;
-    __syncthreads();
-    for (int32_t i = tid; i < count * beams; i += kTraceThreads) {
-      const int32_t t = i / beams, k = i - t * beams;
-      const int32_t p = a.parents[(begin + t) * a.parent_step + group * a.parent_group + k];
-      maps[i] = p >= 0 && p < beams ? static_cast<uint8_t>(p) : kNoBeam;
+    const int32_t* parents = a.parents + begin * a.parent_step + group * a.parent_group + k_own;
+    const int32_t* tokens = a.tokens + begin * a.token_step + group * a.token_group + k_own;
+    if (has_beam) {
+      for (int32_t t = s_own; t < count; t += s_next) copy_word_async(text + t * (beams + 1) + k_own, tokens + t * a.token_step);
+      commit_async();
+#pragma unroll 8
+      for (int32_t t = s_own; t < count; t += s_next) {
+        const int32_t p = __ldg(parents + t * a.parent_step);
+        maps[t * beams + k_own] = p >= 0 && p < beams ? static_cast<uint8_t>(p) : kNoBeam;
+      }
     }
     __syncthreads();
-    for (int32_t i = tid; i < segments * beams; i += kTraceThreads) {
-      const int32_t s = i / beams;
+    for (int32_t s = s_own; s < segments && has_beam; s += s_next) {
       const int32_t t0 = s * a.segment, t1 = min(t0 + a.segment, count);
-      uint8_t at = static_cast<uint8_t>(i - s * beams);
+      int32_t at = k_own;
       for (int32_t t = t1 - 1; t >= t0 && at != kNoBeam; --t) at = maps[t * beams + at];
-      through[i] = at;
+      through[s * beams + k_own] = static_cast<uint8_t>(at);
     }
     __syncthreads();
     if (tid < beams) {
-      uint8_t at = carry[tid];
+      int32_t at = tid;
+      for (int32_t s = segments - 1; s >= 0 && at != kNoBeam; --s) at = through[s * beams + at];
+      whole[tid] = static_cast<uint8_t>(at);
+    }
+    cluster_sync();
+    if (tid < beams) {
+      int32_t at = carry[tid];
+      for (int32_t r = 0; r < rank && at != kNoBeam; ++r) at = peer_byte(whole + at, r);
+      int32_t before = at;  // and on to before the stretch
+      for (int32_t r = rank; r < a.cluster && before != kNoBeam && stop > stretch; ++r) before = peer_byte(whole + before, r);
+      carry[tid] = static_cast<uint8_t>(before);
       for (int32_t s = segments - 1; s >= 0; --s) {
-        enter[s * beams + tid] = at;
+        enter[s * beams + tid] = static_cast<uint8_t>(at);
         if (at != kNoBeam) at = through[s * beams + at];
       }
-      carry[tid] = at;
     }
     __syncthreads();
-    for (int32_t i = tid; i < segments * beams; i += kTraceThreads) {
-      const int32_t s = i / beams, k = i - s * beams;
+    for (int32_t s = s_own; s < segments && has_beam; s += s_next) {
       const int32_t t0 = s * a.segment, t1 = min(t0 + a.segment, count);
-      uint8_t at = enter[i];
+      int32_t at = enter[s * beams + k_own];
       for (int32_t t = t1 - 1; t >= t0; --t) {
-        way[t * beams + k] = at;
+        way[k_own * a.way_stride + t] = static_cast<uint8_t>(at);
         if (at != kNoBeam) at = maps[t * beams + at];
       }
     }
-    __syncthreads();
-    for (int32_t i = tid; i < count * beams; i += kTraceThreads) {
-      const int32_t k = i / count, t = i - k * count;
-      const uint8_t at = way[t * beams + k];
-      out[static_cast<int64_t>(k) * a.steps + begin + t] =
-          at == kNoBeam ? a.pad : a.tokens[(begin + t) * a.token_step + group * a.token_group + at];
+    wait_async<0>();
+    cluster_sync();  // the ways and texts are there, and the window's map has been read by the others
+    for (int32_t k = warp; k < beams; k += kTraceWarps) {
+      int32_t* to = out + static_cast<int64_t>(k) * a.steps + begin;
+      for (int32_t t = lane; t < count; t += 32) {
+        const int32_t at = way[k * a.way_stride + t];
+        to[t] = at == kNoBeam ? a.pad : text[t * (beams + 1) + at];
+      }
     }
+    __syncthreads();
+  }
+  {  // the positions past the end, shared out over the cluster
+    const int32_t left = a.steps - length;
+    for (int32_t k = rank * kTraceWarps + warp; k < beams; k += a.cluster * kTraceWarps)
+      for (int32_t t = lane; t < left; t += 32) out[static_cast<int64_t>(k) * a.steps + length + t] = a.pad;
   }
 }
 
@@ -1305,7 +1437,7 @@ struct Dim {
 // One tensor's rows as at most two outer dimensions over a contiguous run: dimensions of one
 // element drop out, neighbours that continue each other merge (but not across the position
 // dimension's outer side, whose extent differs by group).
-int describe(const XgRowTensor& t, bool has_lengths, int32_t beams, MoveTensor* out, bool* empty) {
+int describe(const XgRowTensor& t, bool has_lengths, MoveTensor* out, bool* empty) {
   const int32_t e = t.element_bytes;
   if (!t.data) return fail(XG_EINVAL, "null tensor");
   if (e != 1 && e != 2 && e != 4 && e != 8 && e != 16) return fail(XG_EINVAL, "elements must have 1, 2, 4, 8 or 16 bytes");
@@ -1376,16 +1508,14 @@ int describe(const XgRowTensor& t, bool has_lengths, int32_t beams, MoveTensor* 
   const int64_t size1 = n == 2 ? d[0].size : 1, size2 = n >= 1 ? d[n - 1].size : 1;
   if (n == 2 && d[0].position) axis = 1;
   if (n >= 1 && d[n - 1].position) axis = 2;
-  // the widest access that everything is a multiple of (16 bytes for 33 beams and more would
-  // take more registers than a thread has)
+  // the widest access that everything is a multiple of
   uint64_t all = reinterpret_cast<uintptr_t>(t.data) | static_cast<uint64_t>(t.rows > 1 ? m.row_bytes : 0) |
                  static_cast<uint64_t>(run) | static_cast<uint64_t>(axis == 3 ? unit : 0) |
                  static_cast<uint64_t>(m.stride1) | static_cast<uint64_t>(m.stride2);
-  int32_t log_bytes = beams > 32 ? 3 : 4;
+  int32_t log_bytes = 4;
   while (all & ((1u << log_bytes) - 1u)) --log_bytes;
   m.log_bytes = log_bytes;
-  if (size1 > 0x7fffffff || size2 > 0x7fffffff || (run >> log_bytes) > 0x7fffffff || (unit >> log_bytes) > 0x7fffffff)
-    return fail(XG_EINVAL, "a row is too large");
+  if (size1 > 0x7fffffff / size2 || (run >> log_bytes) > 0x7fffffff) return fail(XG_EINVAL, "a row is too large");
   m.size1 = static_cast<uint32_t>(size1);
   m.size2 = static_cast<uint32_t>(size2);
   m.size3 = static_cast<uint32_t>(run >> log_bytes);
@@ -1395,24 +1525,21 @@ int describe(const XgRowTensor& t, bool has_lengths, int32_t beams, MoveTensor* 
   return XG_OK;
 }
 
-int launch_moves(const MoveArgs& a, int64_t units, cudaStream_t stream) {
+int launch_moves(const MoveArgs& a, int64_t most_units, cudaStream_t stream) {
   int32_t sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const int64_t tiles = (units + kMoveThreads - 1) / kMoveThreads;
-  int64_t shares = (static_cast<int64_t>(sms) * 16 + a.groups - 1) / a.groups;
-  if (shares > tiles) shares = tiles;
+  static std::atomic<bool> allowed[kDevices];
+  if (int rc = allow_shared(reinterpret_cast<const void*>(move_kernel), kMaxBeams * kMoveThreads * 16, allowed)) return rc;
+  // about one tile a CTA (with 0.6 parents a beam), so that groups with more to move do not hold
+  // the others up; for huge tensors no more CTAs than keep every SM busy many times over
+  const int64_t tile = static_cast<int64_t>(kMoveThreads) * a.slots * 10 / (a.beams * 6 + 4);
+  const int64_t pairs = static_cast<int64_t>(a.groups) * a.count;
+  int64_t shares = (most_units + tile - 1) / tile;
+  const int64_t most = (static_cast<int64_t>(sms) * 128 + pairs - 1) / pairs;
+  if (shares > most) shares = most;
   if (shares < 1) shares = 1;
-  const dim3 grid(static_cast<unsigned>(shares), static_cast<unsigned>(a.groups));
-  if (a.beams <= 4)
-    move_kernel<4><<<grid, kMoveThreads, 0, stream>>>(a);
-  else if (a.beams <= 8)
-    move_kernel<8><<<grid, kMoveThreads, 0, stream>>>(a);
-  else if (a.beams <= 16)
-    move_kernel<16><<<grid, kMoveThreads, 0, stream>>>(a);
-  else if (a.beams <= 32)
-    move_kernel<32><<<grid, kMoveThreads, 0, stream>>>(a);
-  else
-    move_kernel<64><<<grid, kMoveThreads, 0, stream>>>(a);
+  const dim3 grid(static_cast<unsigned>(shares), static_cast<unsigned>(a.groups), static_cast<unsigned>(a.count));
+  move_kernel<<<grid, kMoveThreads, static_cast<size_t>(a.slots) * kMoveThreads * 16, stream>>>(a);
   XG_BEAM_CUDA(cudaGetLastError(), "beam reorder kernel");
   return XG_OK;
 }
@@ -1432,11 +1559,12 @@ int reorder(const XgRowTensor* tensors, int32_t count, const int32_t* parents, i
       return fail(XG_EINVAL, "the tensors need one row per beam");
     MoveTensor m{};
     bool empty = false;
-    if (int rc = describe(tensors[k], lengths != nullptr, beams, &m, &empty)) return rc;
+    if (int rc = describe(tensors[k], lengths != nullptr, &m, &empty)) return rc;
   }
   MoveArgs a{};
   a.groups = groups;
   a.beams = beams;
+  a.slots = beams > kMoveSlots ? beams : kMoveSlots;
   a.rows = tensors[0].rows;
   a.parents = parents;
   a.lengths = lengths;
@@ -1445,9 +1573,10 @@ int reorder(const XgRowTensor* tensors, int32_t count, const int32_t* parents, i
   for (int32_t k = 0; k < count; ++k) {
     bool empty = false;
     MoveTensor& m = a.tensors[a.count];
-    if (int rc = describe(tensors[k], lengths != nullptr, beams, &m, &empty)) return rc;
+    if (int rc = describe(tensors[k], lengths != nullptr, &m, &empty)) return rc;
     if (!empty) {
-      units += static_cast<int64_t>(m.size1) * m.size2 * m.size3;
+      const int64_t of_row = static_cast<int64_t>(m.size1) * m.size2 * m.size3;
+      if (of_row > units) units = of_row;
       ++a.count;
     }
     if (a.count == kMoveTensors || (k + 1 == count && a.count > 0)) {
@@ -1513,6 +1642,7 @@ extern "C" XG_API int xg_beam_sequences(const int32_t* tokens, int64_t token_ste
                                         void* stream) {
   if (steps < 0 || groups < 0 || beams < 1 || beams > kMaxBeams)
     return fail(XG_EINVAL, "a group holds 1 to " + std::to_string(kMaxBeams) + " beams, got " + std::to_string(beams));
+  if (groups > 0x7fffffff / 8) return fail(XG_EINVAL, "too many groups");
   if (steps == 0 || groups == 0) return XG_OK;
   if (!tokens || !parents || !out) return fail(XG_EINVAL, "null argument");
   TraceArgs a{};
@@ -1528,15 +1658,34 @@ extern "C" XG_API int xg_beam_sequences(const int32_t* tokens, int64_t token_ste
   a.lengths = lengths;
   a.pad = pad;
   a.out = out;
-  a.segment = 32;
-  a.window = kTraceBytes / 2 / beams;
-  if (a.window > steps) a.window = steps;
-  const int32_t segments = (a.window + a.segment - 1) / a.segment;
-  const int32_t bytes = 2 * a.window * beams + 2 * segments * beams + beams;
+  // a cluster of up to 8 CTAs a group, each with 64 steps or more of the trace
+  a.cluster = 1;
+  while (a.cluster < 8 && a.cluster * 64 < steps) a.cluster *= 2;
+  a.window = (steps + a.cluster - 1) / a.cluster;
+  const int32_t of_step = 6 * beams + 8;  // bytes, way_stride's rounding included
+  if (a.window > kTraceBytes / of_step) a.window = kTraceBytes / of_step;
+  a.way_stride = (((a.window + 3) / 4) | 1) * 4;  // an odd number of words: beams in different banks
+  a.log_lanes = 0;
+  while ((1 << a.log_lanes) < beams) ++a.log_lanes;
+  // segments of about the square root of the window: the walks inside them and over them are alike
+  a.segment = 8;
+  while (a.segment * a.segment < a.window) a.segment *= 2;
+  a.segments = (a.window + a.segment - 1) / a.segment;
+  const int32_t bytes = a.window * (beams + 1) * 4 + a.window * beams + a.way_stride * beams + 2 * a.segments * beams +
+                        2 * kMaxBeams;
   static std::atomic<bool> allowed[kDevices];
-  if (int rc = allow_shared(reinterpret_cast<const void*>(trace_kernel), kTraceBytes + kTraceBytes / 16 + 1024, allowed)) return rc;
-  trace_kernel<<<static_cast<unsigned>(groups), kTraceThreads, static_cast<size_t>(bytes),
-                 reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  XG_BEAM_CUDA(cudaGetLastError(), "beam sequences kernel");
+  if (int rc = allow_shared(reinterpret_cast<const void*>(trace_kernel), 2 * kTraceBytes, allowed)) return rc;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(groups) * a.cluster);
+  config.blockDim = dim3(kTraceThreads);
+  config.dynamicSmemBytes = static_cast<size_t>(bytes);
+  config.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(a.cluster);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  XG_BEAM_CUDA(cudaLaunchKernelEx(&config, trace_kernel, a), "beam sequences kernel");
   return XG_OK;
 }
