@@ -4,6 +4,7 @@ GPU tests compare with, on worked examples."""
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 import pytest
@@ -60,13 +61,11 @@ def test_sequences_refusals():
 
 def records(*tensors):
     """XgRowTensor records of (rows, row_stride, shape, strides, element_bytes, position[, address])."""
-    from xgraph_b200.beams import _ROW_TENSOR
-
-    out = np.zeros(len(tensors), dtype=_ROW_TENSOR)
-    for r, (rows, row_stride, shape, strides, size, position, *address) in zip(out, tensors):
-        r["data"] = address[0] if address else 1 << 20
-        r["rows"], r["row_stride"], r["dims"], r["element_bytes"], r["position_dim"] = rows, row_stride, len(shape), size, position
-        r["size"][: len(shape)], r["stride"][: len(strides)] = shape, strides
+    out = b""
+    for rows, row_stride, shape, strides, size, position, *address in tensors:
+        pad = (0,) * (4 - len(shape))
+        out += struct.pack("<qqq4q4q4i", address[0] if address else 1 << 20, rows, row_stride, *shape, *pad, *strides,
+                           *pad, len(shape), size, position, 0)
     return out
 
 
@@ -90,16 +89,16 @@ GOOD = (8, 60, (3, 20), (20, 1), 4, -1)
 ])
 def test_reorder_refusals(tensor, message, lengths):
     lib = library()
-    for given in (records(tensor), records((*GOOD[:5], 0), (*tensor[:6], *tensor[6:]))):
-        rc = lib.xg_beam_reorder(given.ctypes.data, len(given), FAKE, 2, 4, lengths, None, None)
-        if message == "one row per beam" and len(given) == 2:
+    for count, given in ((1, records(tensor)), (2, records((*GOOD[:5], 0), tensor))):
+        rc = lib.xg_beam_reorder(given, count, FAKE, 2, 4, lengths, None, None)
+        if message == "one row per beam" and count == 2:
             refused(rc, "same number of rows")
         else:
             refused(rc, message)
     refused(lib.xg_beam_reorder(None, 1, FAKE, 2, 4, None, None, None), "null")
-    refused(lib.xg_beam_reorder(records(GOOD).ctypes.data, 1, None, 2, 4, None, None, None), "null")
-    refused(lib.xg_beam_reorder(records(GOOD).ctypes.data, 1, FAKE, 2, 65, None, None, None), "1 to 64 beams")
-    refused(lib.xg_beam_reorder(records(GOOD).ctypes.data, 1, FAKE, 70000, 4, None, None, None), "groups")
+    refused(lib.xg_beam_reorder(records(GOOD), 1, None, 2, 4, None, None, None), "null")
+    refused(lib.xg_beam_reorder(records(GOOD), 1, FAKE, 2, 65, None, None, None), "1 to 64 beams")
+    refused(lib.xg_beam_reorder(records(GOOD), 1, FAKE, 70000, 4, None, None, None), "groups")
 
 
 def test_null_engine():
@@ -135,21 +134,41 @@ def test_shared_memory_is_found():
 
 
 def test_layouts_of_tensors():
+    """The records have the C structure's layout, and say what the tensors' shapes say."""
     import torch
 
-    from xgraph_b200.beams import _layout, _row_tensors
+    from xgraph_b200.beams import _layout, _load, _row_tensors
 
+    _load()
     cpu = torch.device("cpu")
     a, b = torch.zeros((8, 2, 5), dtype=torch.bfloat16), torch.zeros((8, 4))
-    found, spans = _row_tensors([a, b, a[:, :1]], [2, 1, -1], cpu)
-    assert found["rows"].tolist() == [8, 8, 8] and found["row_stride"].tolist() == [10, 4, 10]
-    assert found["size"].tolist() == [[2, 5, 0, 0], [4, 0, 0, 0], [1, 5, 0, 0]]
-    assert found["position_dim"].tolist() == [1, 0, 1] and found["element_bytes"].tolist() == [2, 4, 2]
-    assert [s[1:] for s in spans] == [(160, True), (128, True), (150, False)]
+    half = torch.zeros((8, 3, 5), dtype=torch.bfloat16)[:, 1:]
+    found, rows = _row_tensors([a, b, half], [2, 1, -1], cpu)
+    assert rows == 8 and len(found) == 3 * 104
+    assert found == records((8, 10, (2, 5), (5, 1), 2, 1, a.data_ptr()), (8, 4, (4,), (1,), 4, 0, b.data_ptr()),
+                            (8, 15, (2, 5), (5, 1), 2, 1, half.data_ptr()))
+    assert [_layout(t, None, cpu)[1:] for t in (a, b, half)] == [(160, True), (128, True), (230, False)]
+    with pytest.raises(ValueError, match="share memory"):
+        _row_tensors([a, b, a], None, cpu)
     for tensor, dim in ((torch.zeros(()), None), (torch.zeros((1,) * 6), None), (a, 0), (a, 3), (a, -3),
                         (torch.zeros((4, 4)).to_sparse(), None)):
         with pytest.raises((ValueError, RuntimeError)):
             _layout(tensor, dim, cpu)
+
+
+def test_the_record_is_the_headers_structure(tmp_path):
+    import subprocess
+    from pathlib import Path
+
+    fields = ("data", "rows", "row_stride", "size", "stride", "dims", "element_bytes", "position_dim", "reserved")
+    prints = "\n".join(f'printf("%zu ", offsetof(XgRowTensor, {f}));' for f in fields)
+    source = tmp_path / "offsets.c"
+    source.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "xgraph_b200.h"\nint main(void) {\n'
+                      + prints + '\nprintf("%zu", sizeof(XgRowTensor));\nreturn 0;\n}\n')
+    include = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run(["gcc", "-std=c11", "-I", str(include), str(source), "-o", str(tmp_path / "offsets")], check=True)
+    printed = subprocess.run([str(tmp_path / "offsets")], check=True, capture_output=True, text=True).stdout
+    assert [int(x) for x in printed.split()] == [0, 8, 16, 24, 56, 88, 92, 96, 100, 104]
 
 
 def test_reference_select_on_a_worked_example():

@@ -23,24 +23,22 @@ its own workspace in the graph's memory.
 from __future__ import annotations
 
 import ctypes
+import struct
 from collections.abc import Sequence
 from contextlib import nullcontext
 from typing import NamedTuple
-
-import numpy as np
 
 MAX_BEAMS = 64
 MAX_CANDIDATES = 128
 MAX_BEAM_VOCAB = 1 << 20
 
-_ROW_TENSOR = np.dtype([  # XgRowTensor
-    ("data", "<i8"), ("rows", "<i8"), ("row_stride", "<i8"), ("size", "<i8", 4), ("stride", "<i8", 4),
-    ("dims", "<i4"), ("element_bytes", "<i4"), ("position_dim", "<i4"), ("reserved", "<i4"),
-])
+# XgRowTensor: data, then rows, row_stride, size[4], stride[4], dims, element_bytes, position_dim, reserved
+_ADDRESS, _ROW_LAYOUT = struct.Struct("<q"), struct.Struct("<qq4q4q4i")
 
 _torch = None
 _lib = None
 _call_errors = None
+_get_device = _get_stream = None  # the current device, and its current raw stream
 _dtypes: dict = {}
 _workspaces: dict[tuple, int] = {}  # bytes a selection of these sizes needs
 
@@ -58,35 +56,32 @@ class BeamCandidates(NamedTuple):
 
 def _load():
     """torch and the library, at the first call (this module imports without either)."""
-    global _torch, _lib, _call_errors
+    global _torch, _lib, _call_errors, _get_device, _get_stream
     if _lib is None:
         import torch
 
         from .engine import _check, load_library
 
         _lib, _call_errors, _torch = load_library(), _check, torch
+        _get_device, _get_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
         _dtypes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
     return _torch
 
 
-def _on_stream(device: int, stream: int):
-    """Allocations of a call belong to the stream its kernels run on."""
-    if _torch._C._cuda_getCurrentRawStream(device) == stream:
-        return nullcontext()
-    if stream == 0:
-        return _torch.cuda.stream(_torch.cuda.default_stream(device))
-    return _torch.cuda.stream(_torch.cuda.ExternalStream(stream, device=device))
-
-
-def _on_device(device: int):
-    return nullcontext() if _torch.cuda.current_device() == device else _torch.cuda.device(device)
+def _placed(device: int, stream: int):
+    """The context in which a call's kernels run on `device` and what it allocates belongs to
+    `stream`; None where that is the current state."""
+    if _get_device() == device and _get_stream(device) == stream:
+        return None
+    return _torch.cuda.stream(_torch.cuda.ExternalStream(stream, device=device) if stream
+                              else _torch.cuda.default_stream(device))
 
 
 def _table(tensor, name: str, shape, dtype, device):
     """A contiguous tensor of this shape and type on `device`; its address."""
     if not isinstance(tensor, _torch.Tensor) or tensor.dtype != dtype or tensor.device != device:
         raise ValueError(f"{name} must be a {str(dtype).removeprefix('torch.')} tensor on {device}")
-    if tuple(tensor.shape) != shape:
+    if tensor.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}, got {list(tensor.shape)}")
     if not tensor.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -143,7 +138,7 @@ def _select(engine, logits, slots, scores, mask, finished, candidates, vocab, en
     elif not 1 <= vocab <= columns:
         raise ValueError(f"vocab must be between 1 and the {columns} columns, got {vocab}")
     wanted = beams if candidates is None else int(candidates)
-    mask_at = mask_stride = 0
+    mask_at, mask_stride = None, 0
     if mask is not None:
         if not isinstance(mask, torch.Tensor) or mask.dtype != torch.int32 or mask.device != device or mask.dim() != 2:
             raise ValueError(f"mask must be a 2-D int32 tensor on {device}")
@@ -163,33 +158,41 @@ def _select(engine, logits, slots, scores, mask, finished, candidates, vocab, en
     if end_token is not None and not 0 <= end_token < vocab:
         raise ValueError(f"end_token must be a token below {vocab}, got {end_token}")
     index = device.index
-    key = (index, groups, beams, vocab, dtype, wanted)
-    with _on_device(index), _on_stream(index, stream):
-        size = _workspaces.get(key)
-        if size is None:
-            out = ctypes.c_int64()
-            _call_errors(_lib.xg_beam_workspace(groups, beams, vocab, dtype, wanted, ctypes.byref(out)))
-            if len(_workspaces) > 4096:
-                _workspaces.clear()
-            size = _workspaces[key] = out.value
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        got = BeamCandidates(
-            torch.empty((groups, wanted), dtype=torch.float32, device=device),
-            torch.empty((groups, wanted), dtype=torch.int32, device=device),
-            torch.empty((groups, wanted), dtype=torch.int32, device=device),
-            torch.empty((groups, wanted), dtype=torch.bool, device=device))
-        tail = (finished_at, wanted, -1 if end_token is None else end_token, 1 if renormalize else 0,
-                got.scores.data_ptr(), got.beams.data_ptr(), got.tokens.data_ptr(), got.finished.data_ptr(),
-                workspace.data_ptr(), size, stream)
-        if engine is None:
-            rc = _lib.xg_beam_select(logits.data_ptr(), dtype, groups, beams, vocab, row_stride, scores_at,
-                                     mask_at or None, mask_stride, *tail)
-        else:
-            rc = _lib.xg_engine_beam_select(engine, logits.data_ptr(), dtype, groups, beams, vocab, row_stride,
-                                            slots, scores_at, *tail)
-        if rc:
-            _call_errors(rc)
-    return got
+    if engine is None:
+        call, head = _lib.xg_beam_select, (logits.data_ptr(), dtype, groups, beams, vocab, row_stride, scores_at,
+                                           mask_at, mask_stride)
+    else:
+        call, head = _lib.xg_engine_beam_select, (engine, logits.data_ptr(), dtype, groups, beams, vocab, row_stride,
+                                                  slots, scores_at)
+    rest = (finished_at, wanted, -1 if end_token is None else end_token, 1 if renormalize else 0)
+    sizes = (index, groups, beams, vocab, dtype, wanted)
+    placed = _placed(index, stream)
+    if placed is None:
+        return _launch_select(call, head, rest, sizes, device, stream)
+    with placed:
+        return _launch_select(call, head, rest, sizes, device, stream)
+
+
+def _launch_select(call, head, rest, sizes, device, stream):
+    size = _workspaces.get(sizes)
+    if size is None:
+        out = ctypes.c_int64()
+        _call_errors(_lib.xg_beam_workspace(*sizes[1:], ctypes.byref(out)))
+        if len(_workspaces) > 4096:
+            _workspaces.clear()
+        size = _workspaces[sizes] = out.value
+    torch, groups, wanted = _torch, sizes[1], sizes[5]
+    empty, shape, strides = torch.empty_strided, (groups, wanted), (wanted, 1)
+    workspace = empty((size,), (1,), dtype=torch.uint8, device=device)
+    scores = empty(shape, strides, dtype=torch.float32, device=device)
+    beams = empty(shape, strides, dtype=torch.int32, device=device)
+    tokens = empty(shape, strides, dtype=torch.int32, device=device)
+    finished = empty(shape, strides, dtype=torch.bool, device=device)
+    rc = call(*head, *rest, scores.data_ptr(), beams.data_ptr(), tokens.data_ptr(), finished.data_ptr(),
+              workspace.data_ptr(), size, stream)
+    if rc:
+        _call_errors(rc)
+    return BeamCandidates(scores, beams, tokens, finished)
 
 
 def beam_reorder(tensors, beams, *, lengths=None, dim: int | Sequence[int] | None = None, rows=None,
@@ -226,43 +229,42 @@ def beam_reorder(tensors, beams, *, lengths=None, dim: int | Sequence[int] | Non
         rows_at = _table(rows, "rows", (groups, per_group), torch.int32, device)
     if not tensors:
         return
-    if dim is None or isinstance(dim, int):
-        dims = [dim] * len(tensors)
-    else:
-        dims = list(dim)
-        if len(dims) != len(tensors):
+    if dim is not None and not isinstance(dim, int):
+        dim = list(dim)
+        if len(dim) != len(tensors):
             raise ValueError("dim needs one entry per tensor")
-    records, spans = _row_tensors(tensors, dims, device)
-    _check_apart(spans)
-    if rows is None and int(records["rows"][0]) != groups * per_group:
-        raise ValueError(f"the tensors need {groups * per_group} rows, one per beam, got {int(records['rows'][0])}")
-    index = device.index
-    with _on_device(index):
-        _call_errors(_lib.xg_beam_reorder(records.ctypes.data, len(records), beams_at, groups, per_group, lengths_at,
-                                          rows_at, stream))
+    records, count = _row_tensors(tensors, dim, device)
+    if rows is None and count != groups * per_group:
+        raise ValueError(f"the tensors need {groups * per_group} rows, one per beam, got {count}")
+    with _placed(device.index, stream) or nullcontext():
+        _call_errors(_lib.xg_beam_reorder(records, len(tensors), beams_at, groups, per_group, lengths_at, rows_at,
+                                          stream))
 
 
-def _row_tensors(tensors, dims, device):
-    """XgRowTensor records, and each tensor's memory as (address, bytes, whether without gaps)."""
-    records = np.zeros(len(tensors), dtype=_ROW_TENSOR)
-    spans, layouts, runs = [], {}, []
-    for tensor, dim in zip(tensors, dims):
+def _row_tensors(tensors, dim, device) -> tuple[bytes, int]:
+    """XgRowTensor records of the tensors, which must not share memory, and the first's rows."""
+    records, spans = [], []
+    shape = stride = dtype = position = None  # of the tensor before: one layout serves a run of alike ones
+    for k, tensor in enumerate(tensors):
         if not isinstance(tensor, _torch.Tensor):
             raise ValueError("tensors must be torch tensors")
-        key = (tensor.shape, tensor.stride(), tensor.dtype, tensor.device, dim)
-        known = layouts.get(key)
-        if known is None:
-            known = layouts[key] = len(layouts), *_layout(tensor, dim, device)
-        runs.append(known[0])
-        spans.append((tensor.data_ptr(), known[2], known[3]))
-    forms = np.array([known[1] for known in layouts.values()], dtype=_ROW_TENSOR)
-    records[:] = forms[0] if len(forms) == 1 else forms[runs]
-    records["data"] = [span[0] for span in spans]
-    return records, spans
+        wanted = dim[k] if isinstance(dim, list) else dim
+        if (k == 0 or tensor.shape != shape or tensor.stride() != stride or tensor.dtype != dtype
+                or tensor.device != device or wanted != position):
+            layout, size, dense = _layout(tensor, wanted, device)
+            shape, stride, dtype, position = tensor.shape, tensor.stride(), tensor.dtype, wanted
+        at = tensor.data_ptr()
+        records.append(_ADDRESS.pack(at))
+        records.append(layout)
+        spans.append((at, size, dense))
+    if len(spans) > 1:
+        _check_apart(spans)
+    return b"".join(records), tensors[0].shape[0]
 
 
-def _layout(tensor, dim, device):
-    """The record (address 0), byte span and density that tensors of this layout share."""
+def _layout(tensor, dim, device) -> tuple[bytes, int, bool]:
+    """What tensors of this layout share: their record after the address, the bytes from the
+    first element to the last, and whether those are all the tensor's."""
     if tensor.device != device:
         raise ValueError(f"the tensors must be on {device}")
     if tensor.dim() < 1 or tensor.dim() > 5:
@@ -281,11 +283,11 @@ def _layout(tensor, dim, device):
         position -= 1
     shape, strides = tensor.shape, tensor.stride()
     pad = (0,) * (4 - count)
-    record = (0, shape[0], strides[0], (*shape[1:], *pad), (*strides[1:], *pad), count, size, position, 0)
+    layout = _ROW_LAYOUT.pack(shape[0], strides[0], *shape[1:], *pad, *strides[1:], *pad, count, size, position, 0)
     if tensor.numel() == 0:
-        return record, 0, True
+        return layout, 0, True
     elements = 1 + sum((n - 1) * s for n, s in zip(shape, strides))
-    return record, elements * size, elements == tensor.numel()
+    return layout, elements * size, elements == tensor.numel()
 
 
 def _check_apart(spans):
@@ -323,9 +325,9 @@ def beam_sequences(tokens, beams, *, lengths=None, pad_token: int = -1, stream: 
     lengths_at = None if lengths is None else _table(lengths, "lengths", (groups,), torch.int32, device)
     if not -(1 << 31) <= pad_token < 1 << 31:
         raise ValueError(f"pad_token must be an int32, got {pad_token}")
-    index = device.index
-    with _on_device(index), _on_stream(index, stream):
-        out = torch.empty((groups, per_group, steps), dtype=torch.int32, device=device)
+    with _placed(device.index, stream) or nullcontext():
+        out = torch.empty_strided((groups, per_group, steps), (per_group * steps, steps, 1), dtype=torch.int32,
+                                  device=device)
         _call_errors(_lib.xg_beam_sequences(
             tokens.data_ptr(), tokens.stride(0), tokens.stride(1), beams.data_ptr(), beams.stride(0), beams.stride(1),
             steps, groups, per_group, lengths_at, pad_token, out.data_ptr(), stream))

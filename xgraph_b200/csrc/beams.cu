@@ -446,6 +446,7 @@ template <typename E, bool MASKED, bool RENORMALIZE>
 __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_constant__ ScanArgs s) {
   extern __shared__ __align__(16) char dynamic[];
   ScanShared& sh = *reinterpret_cast<ScanShared*>(dynamic);
+  asm volatile("griddepcontrol.wait;" ::: "memory");               // what came before on the stream is complete
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge waits for this grid's end
   constexpr int32_t kPer = E::kPer;
   constexpr int32_t kWarpTokens = 32 * kVecs * kPer;  // a warp's vectors of a step are consecutive
@@ -707,13 +708,13 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
 
 constexpr int32_t kMergeThreads = 512;
 constexpr int32_t kMergeWarps = kMergeThreads / 32;
-constexpr int32_t kSamples = 1024;
+constexpr int32_t kMergeKeys = 4;    // keys that a thread loads ahead
+constexpr int32_t kBuckets = 512;    // of 1/16 of a score's unit each
 constexpr double kLn2 = 0.693147180559945309417;
 // Two beams' candidates nearer than this are ordered by log-sums taken again in 64 bits.
 constexpr double kNear = 1e-6;
 
 struct MergeShared {
-  double sample[kSamples];
   double log_sum[kMaxBeams];   // log of the row's sum of exp(x - ref)
   double ref[kMaxBeams];
   double score[kMaxBeams];
@@ -722,13 +723,17 @@ struct MergeShared {
   double best[kMaxCandidates];
   uint32_t best_code[kMaxCandidates];
   double warp_sum[kMergeWarps];
-  double bound;
-  int32_t count, near;
+  unsigned long long warp_most[kMergeWarps], warp_least[kMergeWarps];
+  uint32_t warp_top[kMergeWarps];
+  int32_t counts[2][kMergeWarps];
+  int32_t bucket[kBuckets];          // candidates by their distance from the best
+  uint32_t near_bits[kPoolMax / 32];  // kept candidates with one of another beam too near to tell
+  int32_t count;
 };
 
 // Sum over N_r of exp(x - ref) in 64 bits, by the whole CTA.
 template <typename E>
-__device__ double row_sum(const SelectArgs& a, int32_t row, double ref, double (&scratch)[kMergeWarps]) {
+__device__ __noinline__ double row_sum(const SelectArgs& a, int32_t row, double ref, double (&scratch)[kMergeWarps]) {
   const char* logits = a.logits + static_cast<int64_t>(row) * a.row_stride * E::kBytes;
   const RowMask mask = a.renormalize ? row_mask(a.masks, row) : RowMask{nullptr, nullptr};
   double sum = 0.0;
@@ -753,6 +758,31 @@ __device__ __forceinline__ int32_t split_of(int32_t n) {
   return split;
 }
 
+// Doubles as unsigned integers of the same order.
+__device__ __forceinline__ uint64_t rising(double x) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(x));
+  return b ^ (static_cast<uint64_t>(static_cast<int64_t>(b) >> 63) | 0x8000000000000000ull);
+}
+constexpr uint64_t kRisingNone = 0x000fffffffffffffull;  // rising(-infinity)
+
+__device__ __forceinline__ double from_rising(uint64_t o) {
+  return __longlong_as_double(static_cast<long long>(o ^ ((o >> 63) ? 0x8000000000000000ull : ~0ull)));
+}
+
+// Which sixteenth below the best a score lies in; the last holds all that are farther.
+__device__ __forceinline__ int32_t bucket_of(double score, float best) {
+  const float below = (best - __double2float_rn(score)) * 16.0f;
+  return below < static_cast<float>(kBuckets - 1) ? static_cast<int32_t>(below) : kBuckets - 1;
+}
+
+__device__ __forceinline__ int32_t merge_total(int32_t mine, int32_t (&counts)[kMergeWarps]) {
+  const int32_t of_warp = __reduce_add_sync(kFull, mine);
+  if ((threadIdx.x & 31) == 0) counts[threadIdx.x >> 5] = of_warp;
+  __syncthreads();
+  const int32_t lane = threadIdx.x & 31;
+  return __reduce_add_sync(kFull, lane < kMergeWarps ? counts[lane] : 0);
+}
+
 template <typename E>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ ScanArgs s) {
   extern __shared__ __align__(16) char dynamic[];
@@ -760,24 +790,33 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   const SelectArgs& a = s.a;
   const int32_t pool = s.pool, beams = a.beams, shares = s.shares, wanted = a.candidates;
   double* value = reinterpret_cast<double*>(dynamic);            // [pool]; -inf: none
-  double* kept = value + pool;                                   // [pool] values above the bound,
+  double* kept = value + pool;                                   // [pool] the values that may be among the best
   uint32_t* code = reinterpret_cast<uint32_t*>(kept + pool);     // [pool] beam << 20 | token
   uint32_t* kept_code = code + pool;                             // [pool]
   const int32_t group = blockIdx.x, row0 = group * beams;
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int32_t of_beam = shares * wanted;
+  const uint64_t* keys = s.keys + static_cast<int64_t>(row0) * of_beam;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the scan is complete
 
+  uint64_t ahead[kMergeKeys];
+#pragma unroll
+  for (int32_t k = 0; k < kMergeKeys; ++k) {
+    const int32_t i = tid + k * kMergeThreads;
+    ahead[k] = i < pool ? keys[i] : 0u;
+  }
   for (int32_t b = warp; b < beams; b += kMergeWarps) {
     const int32_t row = row0 + b;
     const float score = a.scores[row];
+    const bool ended = a.finished && a.finished[row];
     int32_t state = 0;
     double ref = 0.0, log_sum = 0.0;
     if (isfinite(score)) {
-      if (a.finished && a.finished[row]) {
+      if (ended) {
         state = 2;
       } else {
         Part p{0.0, 0.0, -CUDART_INF_F, -CUDART_INF_F};
-        for (int32_t c = lane; c < shares; c += 32) {  // at most a few for a lane
+        for (int32_t c = lane; c < shares; c += 32) {  // one for most lanes
           const Part q = s.parts[static_cast<int64_t>(row) * shares + c];
           if (q.anchor != -CUDART_INF_F) {
             const float anchor = fmaxf(p.anchor, q.anchor);
@@ -813,99 +852,166 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       sh.log_sum[b] = log_sum;
     }
   }
-  const int32_t lists = beams * shares;
+  // keep at most so many for the ordering, unless it is all there are
+  const int32_t most_kept = wanted < 32 ? 64 : 2 * wanted;
   for (;;) {
     __syncthreads();
-    for (int32_t i = tid; i < pool; i += kMergeThreads) {
-      const int32_t list = i / wanted, place = i - list * wanted;
-      const int32_t b = list / shares, state = sh.state[b];
+    // every candidate's score
+    uint64_t most = 0, least = ~0ull;
+    bool bisect = false;
+    const auto place = [&](int32_t i, uint64_t key) {
+      const int32_t b = i / of_beam, state = sh.state[b];
       double v = -CUDART_INF;
       int32_t token = 0;
       if (state == 2) {
-        if (place == 0 && list - b * shares == 0 && a.end_token >= 0) {
+        if (i == b * of_beam && a.end_token >= 0) {
           v = sh.score[b];
           token = a.end_token;
         }
-      } else if (state) {
-        const uint64_t key = s.keys[static_cast<int64_t>(row0) * shares * wanted + i];
-        if (key) {
-          token = static_cast<int32_t>(~static_cast<uint32_t>(key));
-          const float x = from_rising(static_cast<uint32_t>(key >> 32));
-          v = sh.score[b] + ((static_cast<double>(x) - sh.ref[b]) - sh.log_sum[b]);
-          if (!isfinite(__double2float_rn(v))) v = -CUDART_INF;
-        }
+      } else if (state && key) {
+        token = static_cast<int32_t>(~static_cast<uint32_t>(key));
+        const float x = from_rising(static_cast<uint32_t>(key >> 32));
+        v = sh.score[b] + ((static_cast<double>(x) - sh.ref[b]) - sh.log_sum[b]);
+        if (!isfinite(__double2float_rn(v))) v = -CUDART_INF;
       }
       value[i] = v;
       code[i] = (static_cast<uint32_t>(b) << 20) | static_cast<uint32_t>(token);
-    }
-    for (int32_t b = tid; b < beams; b += kMergeThreads) sh.again[b] = 0;
-    if (tid == 0) {
-      sh.count = sh.near = 0;
-      sh.bound = -CUDART_INF;
-    }
-    __syncthreads();
-    // a bound that `wanted` candidates reach: the wanted-th best of a sample of distinct ones,
-    // the lists' first places (their maxima over 4 * wanted sets of lists, if there are more)
-    const int32_t target = 4 * wanted;
-    int32_t samples;
-    if (lists >= target) {
-      samples = target;
-      for (int32_t i = tid; i < samples; i += kMergeThreads) {
-        double most = -CUDART_INF;
-        for (int32_t l = i; l < lists; l += target) most = fmax(most, value[l * wanted]);
-        sh.sample[i] = most;
+      if (v != -CUDART_INF) {
+        const uint64_t o = rising(v);
+        most = o > most ? o : most;
+        least = o < least ? o : least;
       }
-    } else {
-      const int32_t places = min((target + lists - 1) / lists, wanted);
-      samples = lists * places;  // fewer than target + lists < 8 * wanted <= kSamples
-      for (int32_t i = tid; i < samples; i += kMergeThreads) {
-        const int32_t l = i / places;
-        sh.sample[i] = value[l * wanted + (i - l * places)];
+    };
+#pragma unroll
+    for (int32_t k = 0; k < kMergeKeys; ++k)
+      if (tid + k * kMergeThreads < pool) place(tid + k * kMergeThreads, ahead[k]);
+    for (int32_t i = tid + kMergeKeys * kMergeThreads; i < pool; i += kMergeThreads) place(i, keys[i]);
+    uint64_t edge = kRisingNone + 1;  // candidates of this order, and with it of a code <= last, and above are kept
+    uint32_t last = kFull;
+    int32_t farthest = kBuckets;      // and at most this far below the best
+    float top_value = 0.0f;
+    if (pool > most_kept) {
+      // the candidates within the fewest sixteenths below the best that hold `wanted`
+      const uint32_t of_warp = __reduce_max_sync(kFull, most ? rising(__double2float_rn(from_rising(most))) : 0u);
+      if (lane == 0) sh.warp_top[warp] = of_warp;
+      for (int32_t i = tid; i < kBuckets; i += kMergeThreads) sh.bucket[i] = 0;
+      __syncthreads();
+      const uint32_t top = __reduce_max_sync(kFull, lane < kMergeWarps ? sh.warp_top[lane] : 0u);
+      top_value = from_rising(top);
+      for (int32_t i = tid; i < pool; i += kMergeThreads)
+        if (value[i] != -CUDART_INF) atomicAdd(&sh.bucket[bucket_of(value[i], top_value)], 1);
+      __syncthreads();
+      constexpr int32_t kEach = kBuckets / 32;
+      int32_t mine = 0;
+#pragma unroll
+      for (int32_t i = 0; i < kEach; ++i) mine += sh.bucket[lane * kEach + i];
+      int32_t upto = mine;
+#pragma unroll
+      for (int32_t d = 1; d < 32; d <<= 1) {
+        const int32_t before = __shfl_up_sync(kFull, upto, d);
+        if (lane >= d) upto += before;
       }
+      const uint32_t enough = __ballot_sync(kFull, upto >= wanted);
+      int32_t level = pool;
+      if (enough) {
+        int32_t at = (__ffs(enough) - 1) * kEach, sum = __shfl_sync(kFull, upto - mine, __ffs(enough) - 1);
+        while ((sum += sh.bucket[at]) < wanted) ++at;
+        level = sum;
+        farthest = at;
+      }
+      bisect = enough && (level > most_kept || farthest == kBuckets - 1);
+      if (bisect) farthest = kBuckets;
     }
-    __syncthreads();
-    {
-      const int32_t split = split_of(samples), step = kMergeThreads / split, part = tid & (split - 1);
-      for (int32_t i0 = 0; i0 < samples; i0 += step) {  // uniform: the shuffles below take whole warps
-        const int32_t i = i0 + tid / split;
-        int32_t rank = 0;
-        const double mine = i < samples ? sh.sample[i] : 0.0;
-        if (i < samples)
-          for (int32_t j = part; j < samples; j += split) {
-            const double other = sh.sample[j];
-            rank += other > mine || (other == mine && j < i);
+    if (bisect) {  // many in one sixteenth, or far from the best: raise the edge by bisection, over
+                   // the bits that the candidates differ in, until few are left above it
+      for (int32_t d = 16; d > 0; d >>= 1) {
+        const uint64_t m = __shfl_xor_sync(kFull, most, d), l = __shfl_xor_sync(kFull, least, d);
+        most = m > most ? m : most;
+        least = l < least ? l : least;
+      }
+      if (lane == 0) {
+        sh.warp_most[warp] = most;
+        sh.warp_least[warp] = least;
+      }
+      __syncthreads();
+      for (int32_t w = 0; w < kMergeWarps; ++w) {
+        most = sh.warp_most[w] > most ? sh.warp_most[w] : most;
+        least = sh.warp_least[w] < least ? sh.warp_least[w] : least;
+      }
+      int32_t turn = 0, level = pool;
+      if (most > least) {
+        const int32_t top_bit = 63 - __clzll(static_cast<long long>(most ^ least));
+        uint64_t base = most & ~((2ull << top_bit) - 1ull);
+        if (top_bit == 63) base = 0;
+        for (int32_t bit = top_bit; bit >= 0 && level > most_kept; --bit, turn ^= 1) {
+          const uint64_t trial = base | (1ull << bit);
+          int32_t mine = 0;
+          for (int32_t i = tid; i < pool; i += kMergeThreads) mine += rising(value[i]) >= trial;
+          const int32_t total = merge_total(mine, sh.counts[turn]);
+          if (total >= wanted) {
+            base = trial;
+            edge = trial;
+            level = total;
           }
-        for (int32_t d = 1; d < split; d <<= 1) rank += __shfl_xor_sync(kFull, rank, d);
-        if (i < samples && part == 0 && rank == wanted - 1) sh.bound = mine;
+        }
+      } else if (most == least) {
+        edge = most;
+      }
+      if (level > most_kept && most >= least) {  // equal scores, or few candidates: by beam and token
+        int32_t above = 0, equal = 0;
+        for (int32_t i = tid; i < pool; i += kMergeThreads) {
+          const uint64_t o = rising(value[i]);
+          above += o > edge;
+          equal += o == edge;
+        }
+        above = merge_total(above, sh.counts[turn]);
+        turn ^= 1;
+        equal = merge_total(equal, sh.counts[turn]);
+        turn ^= 1;
+        if (above + equal > most_kept && above < wanted) {
+          uint32_t before = kFull;  // codes up to before + 1 are kept
+          for (int32_t bit = 25; bit >= 0; --bit, turn ^= 1) {
+            const uint32_t trial = before + (1u << bit);
+            int32_t mine = 0;
+            for (int32_t i = tid; i < pool; i += kMergeThreads) mine += rising(value[i]) == edge && code[i] <= trial;
+            if (merge_total(mine, sh.counts[turn]) < wanted - above) before = trial;
+          }
+          last = before + 1u;
+        }
       }
     }
+    if (tid == 0) sh.count = 0;
+    for (int32_t b = tid; b < beams; b += kMergeThreads) sh.again[b] = 0;
+    for (int32_t i = tid; i < kPoolMax / 32; i += kMergeThreads) sh.near_bits[i] = 0u;
     __syncthreads();
-    const double bound = sh.bound - 2.0 * kNear;
-    for (int32_t i = tid; i < pool; i += kMergeThreads)
-      if (value[i] > -CUDART_INF && value[i] >= bound) {
+    for (int32_t i = tid; i < pool; i += kMergeThreads) {
+      const uint64_t o = rising(value[i]);
+      if (o > kRisingNone && (o > edge || (o == edge && code[i] <= last)) &&
+          (farthest == kBuckets || bucket_of(value[i], top_value) <= farthest)) {
         const int32_t at = atomicAdd(&sh.count, 1);
         kept[at] = value[i];
         kept_code[at] = code[i];
       }
+    }
     __syncthreads();
     const int32_t n = sh.count;
     {
       const int32_t split = split_of(n), step = kMergeThreads / split, part = tid & (split - 1);
-      for (int32_t i0 = 0; i0 < n; i0 += step) {
+      for (int32_t i0 = 0; i0 < n; i0 += step) {  // uniform: the shuffles below take whole warps
         const int32_t i = i0 + tid / split;
         int32_t rank = 0;  // and, from bit 16 on, how many of other beams are too near to tell
         const double mine = i < n ? kept[i] : 0.0;
         const uint32_t own = i < n ? kept_code[i] : 0u;
         if (i < n)
           for (int32_t j = part; j < n; j += split) {
-            const double ahead = kept[j] - mine;
+            const double ahead_by = kept[j] - mine;
             const uint32_t other = kept_code[j];
-            rank += ahead > 0.0 || (ahead == 0.0 && other < own);
-            rank += fabs(ahead) <= kNear && ((other ^ own) >> 20) ? 1 << 16 : 0;
+            rank += ahead_by > 0.0 || (ahead_by == 0.0 && other < own);
+            rank += fabs(ahead_by) <= kNear && ((other ^ own) >> 20) ? 1 << 16 : 0;
           }
         for (int32_t d = 1; d < split; d <<= 1) rank += __shfl_xor_sync(kFull, rank, d);
         if (i < n && part == 0) {
-          if (rank >> 16) sh.near = 1;
+          if (rank >> 16) atomicOr(&sh.near_bits[i >> 5], 1u << (i & 31));
           rank &= 0xffff;
           if (rank < wanted) {
             sh.best[rank] = mine;
@@ -915,25 +1021,29 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
     }
     __syncthreads();
-    if (!sh.near) break;
-    // beams with a candidate that may belong among the best and whose order against another
-    // beam's the 32-bit sums cannot tell
-    const double least = n > wanted ? sh.best[wanted - 1] - kNear : -CUDART_INF;
-    __syncthreads();
-    if (tid == 0) sh.near = 0;
-    __syncthreads();
-    for (int32_t i = tid; i < n; i += kMergeThreads) {
-      const double mine = kept[i];
-      const int32_t own = kept_code[i] >> 20;
-      if (mine < least || sh.state[own] != 1) continue;
-      for (int32_t j = 0; j < n; ++j)
-        if (fabs(kept[j] - mine) <= kNear && static_cast<int32_t>(kept_code[j] >> 20) != own) {
-          sh.again[own] = sh.near = 1;
-          break;
+    // beams whose candidates the 32-bit sums cannot order: among those that may be the best, and
+    // whatever of another beam lies as near to the last of the best
+    bool unsure = false;
+    const auto doubt = [&](uint32_t b) {
+      if (sh.state[b] == 1) {
+        sh.again[b] = 1;
+        unsure = true;
+      }
+    };
+    const double last_best = n >= wanted ? sh.best[wanted - 1] : -CUDART_INF;
+    for (int32_t i = tid; i < n; i += kMergeThreads)
+      if (((sh.near_bits[i >> 5] >> (i & 31)) & 1u) && kept[i] >= last_best - kNear) doubt(kept_code[i] >> 20);
+    if (n >= wanted) {
+      const uint32_t last_beam = sh.best_code[wanted - 1] >> 20;
+      for (int32_t i = tid; i < pool; i += kMergeThreads) {
+        const uint32_t b = code[i] >> 20;
+        if (value[i] >= last_best - kNear && value[i] <= last_best && b != last_beam) {
+          doubt(b);
+          doubt(last_beam);
         }
+      }
     }
-    __syncthreads();
-    if (!sh.near) break;
+    if (!__syncthreads_or(unsure)) break;
     for (int32_t b = 0; b < beams; ++b) {  // at most once for each beam
       if (!sh.again[b]) continue;
       const double sum = row_sum<E>(a, row0 + b, sh.ref[b], sh.warp_sum);
@@ -1380,19 +1490,21 @@ int launch_select(const ScanArgs& s, cudaStream_t stream) {
   if (int rc = allow_shared(reinterpret_cast<const void*>(scan), sizeof(ScanShared),
                             allowed_scan[!masked ? 0 : a.renormalize ? 1 : 2]))
     return rc;
-  scan<<<grid, kScanThreads, sizeof(ScanShared), stream>>>(s);
-  XG_BEAM_CUDA(cudaGetLastError(), "beam scan kernel");
   if (int rc = allow_shared(reinterpret_cast<const void*>(merge_kernel<E>), kPoolMax * 24, allowed)) return rc;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(a.groups));
-  config.blockDim = dim3(kMergeThreads);
-  config.dynamicSmemBytes = static_cast<size_t>(s.pool) * 24;
-  config.stream = stream;
   cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the scan's end
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // a launch overlaps the end of what it waits for
   attribute.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
+  config.stream = stream;
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(kScanThreads);
+  config.dynamicSmemBytes = sizeof(ScanShared);
+  XG_BEAM_CUDA(cudaLaunchKernelEx(&config, scan, s), "beam scan kernel");
+  config.gridDim = dim3(static_cast<unsigned>(a.groups));
+  config.blockDim = dim3(kMergeThreads);
+  config.dynamicSmemBytes = static_cast<size_t>(s.pool) * 24;
   XG_BEAM_CUDA(cudaLaunchKernelEx(&config, merge_kernel<E>, s), "beam merge kernel");
   return XG_OK;
 }
