@@ -243,23 +243,29 @@ def beam_reorder(tensors, beams, *, lengths=None, dim: int | Sequence[int] | Non
 
 def _row_tensors(tensors, dim, device) -> tuple[bytes, int]:
     """XgRowTensor records of the tensors, which must not share memory, and the first's rows."""
+    kind, first = _torch.Tensor, tensors[0]
+    if not isinstance(first, kind):
+        raise ValueError("tensors must be torch tensors")
+    shape, stride, dtype = first.shape, first.stride(), first.dtype
+    if not isinstance(dim, list) and all(
+            [isinstance(t, kind) and t.shape == shape and t.dtype == dtype and t.stride() == stride
+             and t.device == device for t in tensors]):
+        layout, size, dense = _layout(first, dim, device)  # one layout for all, as a model's layers have
+        places = [t.data_ptr() for t in tensors]
+        if len(places) > 1 and size:
+            order = sorted(places)
+            if min([b - a for a, b in zip(order, order[1:])]) < (size if dense else 1):
+                raise ValueError("the tensors share memory")
+        return b"".join([_ADDRESS.pack(at) + layout for at in places]), shape[0]
     records, spans = [], []
-    shape = stride = dtype = position = None  # of the tensor before: one layout serves a run of alike ones
     for k, tensor in enumerate(tensors):
-        if not isinstance(tensor, _torch.Tensor):
+        if not isinstance(tensor, kind):
             raise ValueError("tensors must be torch tensors")
-        wanted = dim[k] if isinstance(dim, list) else dim
-        if (k == 0 or tensor.shape != shape or tensor.stride() != stride or tensor.dtype != dtype
-                or tensor.device != device or wanted != position):
-            layout, size, dense = _layout(tensor, wanted, device)
-            shape, stride, dtype, position = tensor.shape, tensor.stride(), tensor.dtype, wanted
-        at = tensor.data_ptr()
-        records.append(_ADDRESS.pack(at))
-        records.append(layout)
-        spans.append((at, size, dense))
-    if len(spans) > 1:
-        _check_apart(spans)
-    return b"".join(records), tensors[0].shape[0]
+        layout, size, dense = _layout(tensor, dim[k] if isinstance(dim, list) else dim, device)
+        records.append(_ADDRESS.pack(tensor.data_ptr()) + layout)
+        spans.append((tensor.data_ptr(), size, dense))
+    _check_apart(spans)
+    return b"".join(records), shape[0]
 
 
 def _layout(tensor, dim, device) -> tuple[bytes, int, bool]:

@@ -110,12 +110,17 @@ struct Half {  // either 16-bit type
     const uint32_t b = *reinterpret_cast<const uint16_t*>(p);
     w = (k & 1) ? (w & 0x0000ffffu) | (b << 16) : (w & 0xffff0000u) | b;
   }
+  // Four bits spread to the top bits of four bytes by one multiplication, then each copied over
+  // its half of a pair (prmt's sign mode).
   __device__ static void keep(uint4& v, uint32_t bits) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t pair = bits >> (2 * k);
-      const uint32_t m = ((pair & 1u) ? 0x0000ffffu : 0u) | ((pair & 2u) ? 0xffff0000u : 0u);
-      (&v.x)[k] = ((&v.x)[k] & m) | (kNegInf & ~m);
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t spread = ((bits >> (4 * k)) & 15u) * 0x10204080u;
+      uint32_t low, high;
+      asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(low) : "r"(spread));
+      asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(high) : "r"(spread));
+      (&v.x)[2 * k] = ((&v.x)[2 * k] & low) | (kNegInf & ~low);
+      (&v.x)[2 * k + 1] = ((&v.x)[2 * k + 1] & high) | (kNegInf & ~high);
     }
   }
 };
@@ -204,6 +209,12 @@ __device__ __forceinline__ uint64_t make_key(uint32_t order, int32_t token) {
   return (static_cast<uint64_t>(order) << 32) | static_cast<uint32_t>(~token);
 }
 
+// Out of line: a launch's first CTAs wait for every instruction that they reach.
+__device__ __noinline__ double exp_apart(double x) { return exp(x); }
+__device__ __noinline__ uint32_t mask_bits(const RowMask mask, int32_t t0, int32_t n, int32_t vocab) {
+  return mask.bits(t0, n, vocab);
+}
+
 // 2^k of a whole number k <= 0 (0 below the normal doubles), exactly.
 __device__ __forceinline__ double power2(float k) {
   return k < -1000.0f ? 0.0 : __hiloint2double((1023 + static_cast<int32_t>(k)) << 20, 0);
@@ -221,9 +232,10 @@ struct ScanShared {
     uint32_t tops[kRound][kScanThreads];  // rising() of each thread's maximum in each step
     uint64_t pushed[kPushCap];            // afterwards the listed entries' keys
   };
-  uint64_t few[kRankMost];
+  alignas(16) uint64_t few[kRankMost];
   int32_t list[kListCap];              // entries: step of the round * kScanThreads + thread
-  uint32_t thread_top[kScanThreads];   // the threads' maxima in the round
+  uint32_t thread_top[kScanWarps][32];  // the threads' maxima in the round
+  uint32_t warp_bound[2][kScanWarps];
   Part warp_part[kScanWarps];
   int32_t counts[2][kScanWarps];
   int32_t listed, count, few_count;
@@ -240,48 +252,52 @@ __device__ __forceinline__ int32_t block_total(int32_t mine, int32_t (&counts)[k
   return total;
 }
 
+// At most kRankMost of the n keys in sh.pushed, `wanted` best among them: the keys are bisected
+// until few are above the edge.  Returns how many are left.
+__device__ __noinline__ int32_t fewer_keys(ScanShared& sh, int32_t n, int32_t wanted) {
+  const int32_t tid = threadIdx.x;
+  constexpr int32_t kEach = kPushCap / kScanThreads;
+  uint64_t key[kEach], edge = 0;
+#pragma unroll
+  for (int32_t i = 0; i < kEach; ++i) key[i] = tid + i * kScanThreads < n ? sh.pushed[tid + i * kScanThreads] : 0u;
+  int32_t turn = 0;
+#pragma unroll 1
+  for (int32_t bit = 63; bit >= 0; --bit, turn ^= 1) {
+    const uint64_t trial = edge | (1ull << bit);
+    int32_t mine = 0;
+#pragma unroll
+    for (int32_t i = 0; i < kEach; ++i) mine += key[i] >= trial;
+    const int32_t total = block_total(mine, sh.counts[turn]);
+    if (total >= wanted) {
+      edge = trial;
+      if (total <= kRankMost) break;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) sh.few_count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int32_t i = 0; i < kEach; ++i)
+    if (key[i] >= edge && key[i] != 0u) sh.pushed[atomicAdd(&sh.few_count, 1)] = key[i];
+  __syncthreads();
+  return sh.few_count;
+}
+
 // The best min(n, wanted) of the n keys in sh.pushed, in order, into sh.few (all threads; a
 // barrier before the call has made the keys visible and one is passed after them).
 __device__ __forceinline__ int32_t best_of(ScanShared& sh, int32_t n, int32_t wanted) {
-  const int32_t tid = threadIdx.x;
-  constexpr int32_t kEach = kPushCap / kScanThreads;
-  uint64_t edge = 0;
-  if (n > kRankMost) {  // fewer first: bisect the keys until at most kRankMost are above the edge
-    uint64_t key[kEach];
-#pragma unroll
-    for (int32_t i = 0; i < kEach; ++i) key[i] = tid + i * kScanThreads < n ? sh.pushed[tid + i * kScanThreads] : 0u;
-    int32_t turn = 0;
-    for (int32_t bit = 63; bit >= 0; --bit, turn ^= 1) {
-      const uint64_t trial = edge | (1ull << bit);
-      int32_t mine = 0;
-#pragma unroll
-      for (int32_t i = 0; i < kEach; ++i) mine += key[i] >= trial;
-      const int32_t total = block_total(mine, sh.counts[turn]);
-      if (total >= wanted) {
-        edge = trial;
-        if (total <= kRankMost) break;
-      }
-    }
-    __syncthreads();
-    if (tid == 0) sh.few_count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int32_t i = 0; i < kEach; ++i)
-      if (key[i] >= edge && key[i] != 0u) sh.few[atomicAdd(&sh.few_count, 1)] = key[i];
-    __syncthreads();
-    n = sh.few_count;
-    for (int32_t i = tid; i < n; i += kScanThreads) sh.pushed[i] = sh.few[i];
-    __syncthreads();
-  }
-  uint64_t mine = 0;
-  int32_t rank = kRankMost;
-  if (tid < n) {
-    mine = sh.pushed[tid];
-    rank = 0;
+  if (n > kRankMost) n = fewer_keys(sh, n, wanted);
+  // several threads of a warp share a key's comparisons
+  int32_t split = 1;
+  while (split < 32 && n * split * 2 <= kScanThreads) split <<= 1;
+  const int32_t i = threadIdx.x / split;
+  const uint64_t mine = i < n ? sh.pushed[i] : 0u;
+  int32_t rank = 0;
 #pragma unroll 4
-    for (int32_t j = 0; j < n; ++j) rank += sh.pushed[j] > mine;
-  }
-  if (rank < wanted) sh.few[rank] = mine;
+  for (int32_t j = threadIdx.x & (split - 1); j < n; j += split) rank += sh.pushed[j] > mine;
+#pragma unroll 1
+  for (int32_t d = 1; d < split; d <<= 1) rank += __shfl_xor_sync(kFull, rank, d);
+  if (i < n && rank < wanted) sh.few[rank] = mine;  // the same from each of them
   __syncthreads();
   return min(n, wanted);
 }
@@ -352,10 +368,10 @@ __device__ __noinline__ void push_crowded(ScanShared& sh, int32_t vectors, int32
     int32_t mine = 0;
 #pragma unroll 1
     for (int32_t i = tid; i < vectors; i += kScanThreads) {
-      const uint4 v = sh.ring[i];
+      const char* v = reinterpret_cast<const char*>(sh.ring + i);
       const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
-#pragma unroll
-      for (int32_t k = 0; k < kPer; ++k) mine += pick(rising(E::at(v, k) + 0.0f), t0 + k);
+#pragma unroll 2
+      for (int32_t k = 0; k < kPer; ++k) mine += pick(rising(E::one(v + k * E::kBytes) + 0.0f), t0 + k);
     }
     turn ^= 1;
     return block_total(mine, sh.counts[turn]);
@@ -385,11 +401,11 @@ __device__ __noinline__ void push_crowded(ScanShared& sh, int32_t vectors, int32
   __syncthreads();
 #pragma unroll 1
   for (int32_t i = tid; i < vectors; i += kScanThreads) {
-    const uint4 v = sh.ring[i];
+    const char* v = reinterpret_cast<const char*>(sh.ring + i);
     const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
-#pragma unroll
+#pragma unroll 1
     for (int32_t k = 0; k < kPer; ++k) {
-      const uint32_t o = rising(E::at(v, k) + 0.0f);
+      const uint32_t o = rising(E::one(v + k * E::kBytes) + 0.0f);
       if (o >= edge && (o > edge || t0 + k <= last)) {
         const int32_t n = atomicAdd(&sh.count, 1);
         if (n < kPushCap) sh.pushed[n] = make_key(o, t0 + k);
@@ -412,7 +428,7 @@ __device__ __forceinline__ Part total_part(Part p) {
   if (__any_sync(kFull, far != -CUDART_INF_F)) {
 #pragma unroll
     for (int32_t d = 16; d > 0; d >>= 1) far = fmaxf(far, __shfl_xor_sync(kFull, far, d));
-    if (p.far != -CUDART_INF_F) far_sum = p.far_sum * exp(static_cast<double>(p.far) - static_cast<double>(far));
+    if (p.far != -CUDART_INF_F) far_sum = p.far_sum * exp_apart(static_cast<double>(p.far) - static_cast<double>(far));
 #pragma unroll
     for (int32_t d = 16; d > 0; d >>= 1) far_sum += __shfl_xor_sync(kFull, far_sum, d);
   }
@@ -430,16 +446,19 @@ __device__ __forceinline__ void wait_async() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// One vector of a row: tokens t0 .. t0 + kPer, -inf outside [0, vocab).
+// A vector that crosses an end of its row: tokens t0 .. t0 + kPer, -inf outside [0, vocab).
 template <typename E>
-__device__ __forceinline__ uint4 load_vector(const char* logits, int32_t t0, int32_t vocab) {
-  const char* at = logits + static_cast<int64_t>(t0) * E::kBytes;
-  if (t0 >= 0 && t0 + E::kPer <= vocab) return *reinterpret_cast<const uint4*>(at);
+__device__ __noinline__ uint4 load_edge(const char* logits, int32_t t0, int32_t vocab) {
   uint4 v = make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
 #pragma unroll
   for (int32_t k = 0; k < E::kPer; ++k)
-    if (t0 + k >= 0 && t0 + k < vocab) E::put(v, k, at + k * E::kBytes);
+    if (t0 + k >= 0 && t0 + k < vocab) E::put(v, k, logits + static_cast<int64_t>(t0 + k) * E::kBytes);
   return v;
+}
+template <typename E>
+__device__ __forceinline__ uint4 load_vector(const char* logits, int32_t t0, int32_t vocab) {
+  if (t0 >= 0 && t0 + E::kPer <= vocab) return *reinterpret_cast<const uint4*>(logits + static_cast<int64_t>(t0) * E::kBytes);
+  return load_edge<E>(logits, t0, vocab);
 }
 
 template <typename E, bool MASKED, bool RENORMALIZE>
@@ -480,16 +499,19 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
   const auto own_bits = [&](int32_t step, uint32_t word) {
     uint32_t bits = 0u;
     if (head == 0) {
+      if (!__any_sync(kFull, word != 0u)) return 0u;
+      constexpr uint32_t kEvery = kVecs * kPer == 32 ? kFull : (1u << (kVecs * kPer & 31)) - 1u;
+      if (__all_sync(kFull, word == kFull || lane * 32 >= kWarpTokens)) return kEvery;
 #pragma unroll
       for (int32_t j = 0; j < kVecs; ++j) {
         const uint32_t got = __shfl_sync(kFull, word, j * kPer + lane * kPer / 32);
         bits |= ((got >> ((lane * kPer) & 31)) & kAll) << (j * kPer);
       }
     } else if (step < end) {
-#pragma unroll
+#pragma unroll 1
       for (int32_t j = 0; j < kVecs; ++j) {
         const int32_t t0 = warp_token(step) + (j * 32 + lane) * kPer;
-        if (t0 < vocab) bits |= mask.bits(t0, kPer, vocab) << (j * kPer);
+        if (t0 < vocab) bits |= mask_bits(mask, t0, kPer, vocab) << (j * kPer);
       }
     }
     return bits;
@@ -507,7 +529,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
           to[j * kScanThreads] = make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
       }
     } else {
-#pragma unroll
+#pragma unroll 1
       for (int32_t j = 0; j < kVecs; ++j) {
         const int32_t t = t0 + (j * 32 + lane) * kPer;
         if (t < vocab && (!kSkips || ((bits >> (j * kPer)) & kAll)))
@@ -523,38 +545,56 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
   float limit = -CUDART_INF_F;      // logits above it raise the anchor
   int32_t held = 0;                 // best keys of earlier rounds, in sh.few
 
+#pragma unroll 1
   for (int32_t round = begin; round < end; round += kRound) {
     const int32_t stop = min(round + kRound, end);
-    uint32_t bits[kSteps] = {0u, 0u}, word = 0u;
+    uint32_t bits[kSteps] = {0u, 0u};
     if (MASKED) {
       if (!scans) return;
-      const uint32_t word0 = load_word(round), word1 = round + 1 < stop ? load_word(round + 1) : 0u;
-      word = round + 2 < stop ? load_word(round + 2) : 0u;
-      bits[0] = own_bits(round, word0);
-      bits[1] = own_bits(round + 1, word1);
+      // the round's mask words, all in flight together: a step's lie where its maxima will
+#pragma unroll 8
+      for (int32_t k = 0; k < kRound; ++k)
+        if (round + k < stop) sh.tops[k][tid] = load_word(round + k);
+      bits[0] = own_bits(round, sh.tops[0][tid]);
+      if (round + 1 < stop) bits[1] = own_bits(round + 1, sh.tops[1][tid]);
     }
-    issue(round, bits[0], sh.ring + tid);
-    commit_async();
-    if (round + 1 < stop) issue(round + 1, bits[1], sh.ring + kVecs * kScanThreads + tid);
-    commit_async();
+#pragma unroll 1
+    for (int32_t k = 0; k < kSteps; ++k) {
+      if (round + k < stop) issue(round + k, k ? bits[1] : bits[0], sh.ring + k * kVecs * kScanThreads + tid);
+      commit_async();
+    }
     if (!MASKED && !scans) {  // the first loads did not wait for the row's flags
       wait_async<0>();
       return;
     }
     float best = -CUDART_INF_F;  // the thread's best logit that it may take
+#pragma unroll 1
     for (int32_t step = round; step < stop; ++step) {
       wait_async<kSteps - 1>();
       const int32_t at = step - round;
       uint4* slot = sh.ring + (at & 1) * kVecs * kScanThreads + tid;
       const uint32_t own = MASKED ? bits[0] : 0u;
+      constexpr uint32_t kEvery = kVecs * kPer == 32 ? kFull : (1u << (kVecs * kPer & 31)) - 1u;
+      const bool whole = !MASKED || __all_sync(kFull, own == kEvery);  // the warp's every token is allowed
+      const auto next_step = [&]() {  // the slots are read: the step after the next
+        if (MASKED) bits[0] = bits[1];
+        if (step + 2 < stop) {
+          if (MASKED) bits[1] = own_bits(step + 2, sh.tops[at + 2][tid]);
+          issue(step + 2, bits[1], slot);
+        }
+        commit_async();
+      };
+      if (kSkips && !__any_sync(kFull, own != 0u)) {  // none of the warp's tokens is
+        sh.tops[at][tid] = kRisingLowest - 1u;
+        next_step();
+        continue;
+      }
       uint4 v[kVecs];
 #pragma unroll
-      for (int32_t j = 0; j < kVecs; ++j) {
-        v[j] = slot[j * kScanThreads];
-        if (kSkips) {
-          const uint32_t b = (own >> (j * kPer)) & kAll;
-          if (b != kAll) E::keep(v[j], b);
-        }
+      for (int32_t j = 0; j < kVecs; ++j) v[j] = slot[j * kScanThreads];
+      if (kSkips && !whole) {
+#pragma unroll
+        for (int32_t j = 0; j < kVecs; ++j) E::keep(v[j], (own >> (j * kPer)) & kAll);
       }
       float shown = E::top(v);
       bool far_step = false;
@@ -576,18 +616,20 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
       if (far_step) {  // so far from 0 that log2 e's rounding would show: the difference comes first
         const float most = from_rising(__reduce_max_sync(kFull, rising(shown)));
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
+#pragma unroll 1
         for (int32_t j = 0; j < kVecs; ++j) {
+          uint4 x = slot[j * kScanThreads];
+          if (kSkips) E::keep(x, (own >> (j * kPer)) & kAll);
 #pragma unroll
           for (int32_t k = 0; k < kPer; ++k) {
-            const float d = E::at(v[j], k) - most;
+            const float d = E::at(x, k) - most;
             acc[k & 3] += exp2_fast(fmaf(d, kLog2eHi, d * kLog2eLo));
           }
         }
         const double part = static_cast<double>((acc[0] + acc[1]) + (acc[2] + acc[3]));
         const float higher = fmaxf(far, most);
-        far_sum = (far == -CUDART_INF_F ? 0.0 : far_sum * exp(static_cast<double>(far) - static_cast<double>(higher))) +
-                  part * exp(static_cast<double>(most) - static_cast<double>(higher));
+        far_sum = (far == -CUDART_INF_F ? 0.0 : far_sum * exp_apart(static_cast<double>(far) - static_cast<double>(higher))) +
+                  part * exp_apart(static_cast<double>(most) - static_cast<double>(higher));
         far = higher;
       } else if (anchor != -CUDART_INF_F) {
         // exp(x) as 2^(x log2 e - anchor) with a whole anchor near the maximum: sums of
@@ -596,7 +638,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
         uint64_t acc[2] = {0, 0};
 #pragma unroll
         for (int32_t j = 0; j < kVecs; ++j) {
-          if (kSkips && !__any_sync(kFull, (own >> (j * kPer)) & kAll)) continue;
+          if (kSkips && !whole && !__any_sync(kFull, (own >> (j * kPer)) & kAll)) continue;
 #pragma unroll
           for (int32_t k = 0; k < kPer; k += 2) {
             const uint64_t x = pack2(E::at(v[j], k), E::at(v[j], k + 1));
@@ -607,54 +649,61 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
         const uint64_t all = add2(acc[0], acc[1]);
         sum += static_cast<double>(low(all) + high(all));
       }
-      if (MASKED && !RENORMALIZE) {
+      if (MASKED && !RENORMALIZE && !whole) {
 #pragma unroll
-        for (int32_t j = 0; j < kVecs; ++j) {
-          const uint32_t b = (own >> (j * kPer)) & kAll;
-          if (b != kAll) E::keep(v[j], b);
-        }
+        for (int32_t j = 0; j < kVecs; ++j) E::keep(v[j], (own >> (j * kPer)) & kAll);
         shown = E::top(v);
       }
       sh.tops[at][tid] = rising(shown + 0.0f);
       best = fmaxf(best, shown);
-      // the slots are read: the step after the next
-      if (MASKED) {
-        bits[0] = bits[1];
-        bits[1] = own_bits(step + 2, word);
-        word = step + 3 < stop ? load_word(step + 3) : 0u;
-      }
-      if (step + 2 < stop) issue(step + 2, bits[1], slot);
-      commit_async();
+      next_step();
     }
 
-    // the best tokens of the round and of the keys held: the entries that reach the wanted-th of
-    // the threads' maxima (to its upper 16 bits) or, once enough are held, the last of them
+    // the best tokens of the round and of the keys held: the entries that reach a bound which
+    // `wanted` tokens reach -- the least, over the warps, of a warp's (wanted / 8)-th best thread,
+    // or one warp's own wanted-th best, whichever is more -- and, once enough keys are held, more
+    // than the last of them
     const int32_t steps = stop - round;
     const int32_t first = round * kStepTokens - head;
-    sh.thread_top[tid] = rising(best + 0.0f);
-    if (tid == 0) sh.listed = 0;
-    __syncthreads();
-    uint32_t bound = 0;
     {
-      uint32_t of[kScanThreads / 32];
+      const uint32_t mine = rising(best + 0.0f);
+      sh.thread_top[warp][lane] = mine;
+      __syncwarp();
+      int32_t rank = 0;
 #pragma unroll
-      for (int32_t i = 0; i < kScanThreads / 32; ++i) of[i] = sh.thread_top[i * 32 + lane];
-#pragma unroll 1
-      for (int32_t bit = 31; bit >= 16; --bit) {
-        const uint32_t trial = bound | (1u << bit);
-        int32_t reached = 0;
-#pragma unroll
-        for (int32_t i = 0; i < kScanThreads / 32; ++i) reached += of[i] >= trial;
-        if (__reduce_add_sync(kFull, reached) >= wanted) bound = trial;
+      for (int32_t k = 0; k < 8; ++k) {
+        const uint4 other = reinterpret_cast<const uint4*>(sh.thread_top[warp])[k];
+        rank += (other.x > mine) + (other.y > mine) + (other.z > mine) + (other.w > mine);
+      }
+      rank += __popc(__match_any_sync(kFull, mine) & ((1u << lane) - 1u));  // equal ones by lane
+      const uint32_t of_all = __reduce_max_sync(kFull, rank == (wanted + kScanWarps - 1) / kScanWarps - 1 ? mine : 0u);
+      const uint32_t of_one = __reduce_max_sync(kFull, rank == wanted - 1 ? mine : 0u);
+      if (lane == 0) {
+        sh.warp_bound[0][warp] = of_all;
+        sh.warp_bound[1][warp] = of_one;
       }
     }
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    uint32_t bound = kFull, alone = 0;
+#pragma unroll
+    for (int32_t w = 0; w < kScanWarps; ++w) {
+      bound = min(bound, sh.warp_bound[0][w]);
+      alone = max(alone, sh.warp_bound[1][w]);
+    }
+    bound = max(bound, alone);
     bound = max(bound, kRisingLowest);
     if (held == wanted) bound = max(bound, static_cast<uint32_t>(sh.few[wanted - 1] >> 32) + 1u);
-    for (int32_t at = 0; at < steps; ++at)
-      if (sh.tops[at][tid] >= bound) {
+    if (rising(best + 0.0f) >= bound) {
+      uint32_t reached = 0;  // steps
+#pragma unroll 4
+      for (int32_t at = 0; at < steps; ++at) reached |= sh.tops[at][tid] >= bound ? 1u << at : 0u;
+#pragma unroll 1
+      for (; reached; reached &= reached - 1u) {
         const int32_t n = atomicAdd(&sh.listed, 1);
-        if (n < kListCap) sh.list[n] = at * kScanThreads + tid;
+        if (n < kListCap) sh.list[n] = (__ffs(reached) - 1) * kScanThreads + tid;
       }
+    }
     __syncthreads();
     if (sh.listed > kListCap) bound = max(bound, list_crowded(sh, steps, wanted));
     const int32_t vectors = min(sh.listed, kListCap) * kVecs;
@@ -663,22 +712,26 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
     __syncthreads();
     const float least = from_rising(bound);
     bool over = false;
+#pragma unroll 1
     for (int32_t i = tid; i < vectors; i += kScanThreads) {
       const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
       uint4 v = make_uint4(E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf);
       if (t0 < vocab) {
         v = load_vector<E>(logits, t0, vocab);
-        if (MASKED) E::keep(v, mask.bits(t0, kPer, vocab));
+        if (MASKED && !mask.all())
+          E::keep(v, head == 0 ? (mask.word(t0 >> 5) >> (t0 & 31)) & kAll : mask_bits(mask, t0, kPer, vocab));
       }
       sh.ring[i] = v;
+      uint32_t reached = 0;
 #pragma unroll
-      for (int32_t k = 0; k < kPer; ++k) {
-        const float x = E::at(v, k) + 0.0f;
-        if (x >= least) {
-          const int32_t n = atomicAdd(&sh.count, 1);
-          if (n < kPushCap) sh.pushed[n] = make_key(rising(x), t0 + k);
-          over |= n >= kPushCap;
-        }
+      for (int32_t k = 0; k < kPer; ++k) reached |= E::at(v, k) >= least ? 1u << k : 0u;
+#pragma unroll 1
+      for (; reached; reached &= reached - 1u) {
+        const int32_t k = __ffs(reached) - 1;
+        const float x = E::one(reinterpret_cast<const char*>(sh.ring + i) + k * E::kBytes) + 0.0f;
+        const int32_t n = atomicAdd(&sh.count, 1);
+        if (n < kPushCap) sh.pushed[n] = make_key(rising(x), t0 + k);
+        over |= n >= kPushCap;
       }
     }
     if (__syncthreads_or(over)) push_crowded<E>(sh, vectors, first, held, wanted);
@@ -693,6 +746,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
   }
   if (lane == 0) sh.warp_part[warp] = Part{sum, far_sum, anchor, far};
   uint64_t* out = s.keys + static_cast<int64_t>(blockIdx.x) * wanted;
+#pragma unroll 1
   for (int32_t i = tid; i < wanted; i += kScanThreads) out[i] = i < held ? sh.few[i] : 0u;
   __syncthreads();
   if (warp == 0) {
@@ -737,6 +791,7 @@ __device__ __noinline__ double row_sum(const SelectArgs& a, int32_t row, double 
   const char* logits = a.logits + static_cast<int64_t>(row) * a.row_stride * E::kBytes;
   const RowMask mask = a.renormalize ? row_mask(a.masks, row) : RowMask{nullptr, nullptr};
   double sum = 0.0;
+#pragma unroll 1
   for (int32_t t = threadIdx.x; t < a.vocab; t += kMergeThreads) {
     if (!mask.all() && !((mask.word(t >> 5) >> (t & 31)) & 1u)) continue;
     sum += exp(static_cast<double>(E::one(logits + static_cast<int64_t>(t) * E::kBytes)) - ref);
@@ -746,6 +801,7 @@ __device__ __noinline__ double row_sum(const SelectArgs& a, int32_t row, double 
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
   __syncthreads();
   sum = 0.0;
+#pragma unroll 1
   for (int32_t w = 0; w < kMergeWarps; ++w) sum += scratch[w];
   __syncthreads();
   return sum;
@@ -805,6 +861,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     const int32_t i = tid + k * kMergeThreads;
     ahead[k] = i < pool ? keys[i] : 0u;
   }
+#pragma unroll 1
   for (int32_t b = warp; b < beams; b += kMergeWarps) {
     const int32_t row = row0 + b;
     const float score = a.scores[row];
@@ -816,6 +873,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         state = 2;
       } else {
         Part p{0.0, 0.0, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll 1
         for (int32_t c = lane; c < shares; c += 32) {  // one for most lanes
           const Part q = s.parts[static_cast<int64_t>(row) * shares + c];
           if (q.anchor != -CUDART_INF_F) {
@@ -825,8 +883,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
           }
           if (q.far != -CUDART_INF_F) {
             const float far = fmaxf(p.far, q.far);
-            p.far_sum = (p.far == -CUDART_INF_F ? 0.0 : p.far_sum * exp(static_cast<double>(p.far) - static_cast<double>(far))) +
-                        q.far_sum * exp(static_cast<double>(q.far) - static_cast<double>(far));
+            p.far_sum = (p.far == -CUDART_INF_F ? 0.0 : p.far_sum * exp_apart(static_cast<double>(p.far) - static_cast<double>(far))) +
+                        q.far_sum * exp_apart(static_cast<double>(q.far) - static_cast<double>(far));
             p.far = far;
           }
         }
@@ -836,7 +894,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         if (p.far != -CUDART_INF_F) {
           const double far = static_cast<double>(p.far);
           const double higher = p.anchor == -CUDART_INF_F || far > ref ? far : ref;
-          sum = (p.anchor == -CUDART_INF_F ? 0.0 : sum * exp(ref - higher)) + p.far_sum * exp(far - higher);
+          sum = (p.anchor == -CUDART_INF_F ? 0.0 : sum * exp_apart(ref - higher)) + p.far_sum * exp_apart(far - higher);
           ref = higher;
         }
         if (isfinite(sum) && sum > 0.0) {
@@ -885,6 +943,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
 #pragma unroll
     for (int32_t k = 0; k < kMergeKeys; ++k)
       if (tid + k * kMergeThreads < pool) place(tid + k * kMergeThreads, ahead[k]);
+#pragma unroll 1
     for (int32_t i = tid + kMergeKeys * kMergeThreads; i < pool; i += kMergeThreads) place(i, keys[i]);
     uint64_t edge = kRisingNone + 1;  // candidates of this order, and with it of a code <= last, and above are kept
     uint32_t last = kFull;
@@ -894,10 +953,12 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       // the candidates within the fewest sixteenths below the best that hold `wanted`
       const uint32_t of_warp = __reduce_max_sync(kFull, most ? rising(__double2float_rn(from_rising(most))) : 0u);
       if (lane == 0) sh.warp_top[warp] = of_warp;
+#pragma unroll 1
       for (int32_t i = tid; i < kBuckets; i += kMergeThreads) sh.bucket[i] = 0;
       __syncthreads();
       const uint32_t top = __reduce_max_sync(kFull, lane < kMergeWarps ? sh.warp_top[lane] : 0u);
       top_value = from_rising(top);
+#pragma unroll 1
       for (int32_t i = tid; i < pool; i += kMergeThreads)
         if (value[i] != -CUDART_INF) atomicAdd(&sh.bucket[bucket_of(value[i], top_value)], 1);
       __syncthreads();
@@ -934,6 +995,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         sh.warp_least[warp] = least;
       }
       __syncthreads();
+#pragma unroll 1
       for (int32_t w = 0; w < kMergeWarps; ++w) {
         most = sh.warp_most[w] > most ? sh.warp_most[w] : most;
         least = sh.warp_least[w] < least ? sh.warp_least[w] : least;
@@ -943,9 +1005,11 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         const int32_t top_bit = 63 - __clzll(static_cast<long long>(most ^ least));
         uint64_t base = most & ~((2ull << top_bit) - 1ull);
         if (top_bit == 63) base = 0;
+#pragma unroll 1
         for (int32_t bit = top_bit; bit >= 0 && level > most_kept; --bit, turn ^= 1) {
           const uint64_t trial = base | (1ull << bit);
           int32_t mine = 0;
+#pragma unroll 1
           for (int32_t i = tid; i < pool; i += kMergeThreads) mine += rising(value[i]) >= trial;
           const int32_t total = merge_total(mine, sh.counts[turn]);
           if (total >= wanted) {
@@ -959,6 +1023,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
       if (level > most_kept && most >= least) {  // equal scores, or few candidates: by beam and token
         int32_t above = 0, equal = 0;
+#pragma unroll 1
         for (int32_t i = tid; i < pool; i += kMergeThreads) {
           const uint64_t o = rising(value[i]);
           above += o > edge;
@@ -970,9 +1035,11 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         turn ^= 1;
         if (above + equal > most_kept && above < wanted) {
           uint32_t before = kFull;  // codes up to before + 1 are kept
+#pragma unroll 1
           for (int32_t bit = 25; bit >= 0; --bit, turn ^= 1) {
             const uint32_t trial = before + (1u << bit);
             int32_t mine = 0;
+#pragma unroll 1
             for (int32_t i = tid; i < pool; i += kMergeThreads) mine += rising(value[i]) == edge && code[i] <= trial;
             if (merge_total(mine, sh.counts[turn]) < wanted - above) before = trial;
           }
@@ -981,9 +1048,12 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
     }
     if (tid == 0) sh.count = 0;
+#pragma unroll 1
     for (int32_t b = tid; b < beams; b += kMergeThreads) sh.again[b] = 0;
+#pragma unroll 1
     for (int32_t i = tid; i < kPoolMax / 32; i += kMergeThreads) sh.near_bits[i] = 0u;
     __syncthreads();
+#pragma unroll 1
     for (int32_t i = tid; i < pool; i += kMergeThreads) {
       const uint64_t o = rising(value[i]);
       if (o > kRisingNone && (o > edge || (o == edge && code[i] <= last)) &&
@@ -997,18 +1067,21 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     const int32_t n = sh.count;
     {
       const int32_t split = split_of(n), step = kMergeThreads / split, part = tid & (split - 1);
+#pragma unroll 1
       for (int32_t i0 = 0; i0 < n; i0 += step) {  // uniform: the shuffles below take whole warps
         const int32_t i = i0 + tid / split;
         int32_t rank = 0;  // and, from bit 16 on, how many of other beams are too near to tell
         const double mine = i < n ? kept[i] : 0.0;
         const uint32_t own = i < n ? kept_code[i] : 0u;
         if (i < n)
+#pragma unroll 1
           for (int32_t j = part; j < n; j += split) {
             const double ahead_by = kept[j] - mine;
             const uint32_t other = kept_code[j];
             rank += ahead_by > 0.0 || (ahead_by == 0.0 && other < own);
             rank += fabs(ahead_by) <= kNear && ((other ^ own) >> 20) ? 1 << 16 : 0;
           }
+#pragma unroll 1
         for (int32_t d = 1; d < split; d <<= 1) rank += __shfl_xor_sync(kFull, rank, d);
         if (i < n && part == 0) {
           if (rank >> 16) atomicOr(&sh.near_bits[i >> 5], 1u << (i & 31));
@@ -1031,10 +1104,12 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
     };
     const double last_best = n >= wanted ? sh.best[wanted - 1] : -CUDART_INF;
+#pragma unroll 1
     for (int32_t i = tid; i < n; i += kMergeThreads)
       if (((sh.near_bits[i >> 5] >> (i & 31)) & 1u) && kept[i] >= last_best - kNear) doubt(kept_code[i] >> 20);
     if (n >= wanted) {
       const uint32_t last_beam = sh.best_code[wanted - 1] >> 20;
+#pragma unroll 1
       for (int32_t i = tid; i < pool; i += kMergeThreads) {
         const uint32_t b = code[i] >> 20;
         if (value[i] >= last_best - kNear && value[i] <= last_best && b != last_beam) {
@@ -1044,6 +1119,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
     }
     if (!__syncthreads_or(unsure)) break;
+#pragma unroll 1
     for (int32_t b = 0; b < beams; ++b) {  // at most once for each beam
       if (!sh.again[b]) continue;
       const double sum = row_sum<E>(a, row0 + b, sh.ref[b], sh.warp_sum);
@@ -1053,6 +1129,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
     }
   }
+#pragma unroll 1
   for (int32_t i = tid; i < wanted; i += kMergeThreads) {
     const int64_t to = static_cast<int64_t>(group) * wanted + i;
     float score = -CUDART_INF_F;
@@ -1469,7 +1546,10 @@ int plan(int32_t groups, int32_t beams, int32_t vocab, int32_t dtype, int32_t ca
   const int32_t step = kScanThreads * kVecs * per;  // a misaligned row's vectors start up to a vector early
   const int32_t tiles = (vocab + per - 1 + step - 1) / step;
   const int64_t rows = static_cast<int64_t>(groups) * beams;
-  int64_t shares = rows > 0 ? (static_cast<int64_t>(sms) * 4 + rows - 1) / rows : 1;
+  // one wave of CTAs (four on an SM), but at least two shares of a row unless there are many rows,
+  // so that no SM ends with a whole row more than the others
+  int64_t shares = rows > 0 ? static_cast<int64_t>(sms) * 4 / rows : 1;
+  if (shares < 2 && rows < static_cast<int64_t>(sms) * 8) shares = 2;
   if (shares > kPoolMax / (beams * candidates)) shares = kPoolMax / (beams * candidates);
   if (shares > tiles) shares = tiles;
   if (shares < 1) shares = 1;
@@ -1665,15 +1745,7 @@ int reorder(const XgRowTensor* tensors, int32_t count, const int32_t* parents, i
   if (groups > 65535) return fail(XG_EINVAL, "at most 65535 groups");
   if (count == 0 || groups == 0) return XG_OK;
   if (!tensors || !parents) return fail(XG_EINVAL, "null argument");
-  for (int32_t k = 0; k < count; ++k) {  // every descriptor is checked before the first launch
-    if (tensors[k].rows != tensors[0].rows) return fail(XG_EINVAL, "the tensors of a call have the same number of rows");
-    if (tensors[k].rows < (rows ? 0 : static_cast<int64_t>(groups) * beams) || tensors[k].rows > 0x7fffffff)
-      return fail(XG_EINVAL, "the tensors need one row per beam");
-    MoveTensor m{};
-    bool empty = false;
-    if (int rc = describe(tensors[k], lengths != nullptr, &m, &empty)) return rc;
-  }
-  MoveArgs a{};
+  MoveArgs a;
   a.groups = groups;
   a.beams = beams;
   a.slots = beams > kMoveSlots ? beams : kMoveSlots;
@@ -1681,20 +1753,27 @@ int reorder(const XgRowTensor* tensors, int32_t count, const int32_t* parents, i
   a.parents = parents;
   a.lengths = lengths;
   a.row_of = rows;
-  int64_t units = 0;
-  for (int32_t k = 0; k < count; ++k) {
-    bool empty = false;
-    MoveTensor& m = a.tensors[a.count];
-    if (int rc = describe(tensors[k], lengths != nullptr, &m, &empty)) return rc;
-    if (!empty) {
-      const int64_t of_row = static_cast<int64_t>(m.size1) * m.size2 * m.size3;
-      if (of_row > units) units = of_row;
-      ++a.count;
-    }
-    if (a.count == kMoveTensors || (k + 1 == count && a.count > 0)) {
-      if (int rc = launch_moves(a, units, stream)) return rc;
-      a.count = 0;
-      units = 0;
+  for (int32_t launches = 0; launches < 2; ++launches) {  // every descriptor is checked before the first launch
+    a.count = 0;
+    int64_t most_units = 0;
+    for (int32_t k = 0; k < count; ++k) {
+      if (tensors[k].rows != tensors[0].rows) return fail(XG_EINVAL, "the tensors of a call have the same number of rows");
+      if (tensors[k].rows < (rows ? 0 : static_cast<int64_t>(groups) * beams) || tensors[k].rows > 0x7fffffff)
+        return fail(XG_EINVAL, "the tensors need one row per beam");
+      MoveTensor& m = a.tensors[a.count];
+      bool empty = false;
+      if (int rc = describe(tensors[k], lengths != nullptr, &m, &empty)) return rc;
+      if (!empty) {
+        const int64_t units = static_cast<int64_t>(m.size1) * m.size2 * m.size3;
+        if (units > most_units) most_units = units;
+        ++a.count;
+      }
+      if (a.count == kMoveTensors || (k + 1 == count && a.count > 0)) {
+        if (launches)
+          if (int rc = launch_moves(a, most_units, stream)) return rc;
+        a.count = 0;
+        most_units = 0;
+      }
     }
   }
   return XG_OK;
