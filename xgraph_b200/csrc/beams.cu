@@ -415,22 +415,20 @@ __device__ __noinline__ void push_crowded(ScanShared& sh, int32_t vectors, int32
   __syncthreads();
 }
 
-// The parts of a warp's lanes as one (in every lane).
-__device__ __forceinline__ Part total_part(Part p) {
-  float anchor = p.anchor;
-#pragma unroll
-  for (int32_t d = 16; d > 0; d >>= 1) anchor = fmaxf(anchor, __shfl_xor_sync(kFull, anchor, d));
+// The parts of a warp's first `width` lanes (a power of two; the others hold none) as one, in
+// those lanes.
+__device__ __forceinline__ Part total_part(Part p, int32_t width) {
+  const float anchor = from_rising(__reduce_max_sync(kFull, rising(p.anchor)));
   double sum = p.anchor == -CUDART_INF_F ? 0.0 : p.sum * power2(p.anchor - anchor);
-#pragma unroll
-  for (int32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+#pragma unroll 1
+  for (int32_t d = 1; d < width; d <<= 1) sum += __shfl_xor_sync(kFull, sum, d);
   float far = p.far;
   double far_sum = 0.0;
   if (__any_sync(kFull, far != -CUDART_INF_F)) {
-#pragma unroll
-    for (int32_t d = 16; d > 0; d >>= 1) far = fmaxf(far, __shfl_xor_sync(kFull, far, d));
+    far = from_rising(__reduce_max_sync(kFull, rising(far)));
     if (p.far != -CUDART_INF_F) far_sum = p.far_sum * exp_apart(static_cast<double>(p.far) - static_cast<double>(far));
-#pragma unroll
-    for (int32_t d = 16; d > 0; d >>= 1) far_sum += __shfl_xor_sync(kFull, far_sum, d);
+#pragma unroll 1
+    for (int32_t d = 1; d < width; d <<= 1) far_sum += __shfl_xor_sync(kFull, far_sum, d);
   }
   return Part{sum, far_sum, anchor, far};
 }
@@ -751,7 +749,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
   __syncthreads();
   if (warp == 0) {
     Part p = lane < kScanWarps ? sh.warp_part[lane] : Part{0.0, 0.0, -CUDART_INF_F, -CUDART_INF_F};
-    p = total_part(p);
+    p = total_part(p, kScanWarps);
     if (lane == 0) s.parts[blockIdx.x] = p;
   }
 }
@@ -763,6 +761,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
 constexpr int32_t kMergeThreads = 512;
 constexpr int32_t kMergeWarps = kMergeThreads / 32;
 constexpr int32_t kMergeKeys = 4;    // keys that a thread loads ahead
+constexpr int32_t kDirect = 128;     // so many candidates are put in order without a selection before
 constexpr int32_t kBuckets = 512;    // of 1/16 of a score's unit each
 constexpr double kLn2 = 0.693147180559945309417;
 // Two beams' candidates nearer than this are ordered by log-sums taken again in 64 bits.
@@ -774,14 +773,13 @@ struct MergeShared {
   double score[kMaxBeams];
   int32_t state[kMaxBeams];    // 0 offers nothing, 1 candidates, 2 ended, 3 candidates, 64-bit sum
   int32_t again[kMaxBeams];
-  double best[kMaxCandidates];
+  uint64_t best[kMaxCandidates];  // rising() of the best scores, and their codes
   uint32_t best_code[kMaxCandidates];
   double warp_sum[kMergeWarps];
   unsigned long long warp_most[kMergeWarps], warp_least[kMergeWarps];
   uint32_t warp_top[kMergeWarps];
   int32_t counts[2][kMergeWarps];
   int32_t bucket[kBuckets];          // candidates by their distance from the best
-  uint32_t near_bits[kPoolMax / 32];  // kept candidates with one of another beam too near to tell
   int32_t count;
 };
 
@@ -805,13 +803,6 @@ __device__ __noinline__ double row_sum(const SelectArgs& a, int32_t row, double 
   for (int32_t w = 0; w < kMergeWarps; ++w) sum += scratch[w];
   __syncthreads();
   return sum;
-}
-
-// How many threads of a warp share one item's comparisons with n others.
-__device__ __forceinline__ int32_t split_of(int32_t n) {
-  int32_t split = 1;
-  while (split < 32 && n * split * 2 <= kMergeThreads) split <<= 1;
-  return split;
 }
 
 // Doubles as unsigned integers of the same order.
@@ -839,16 +830,148 @@ __device__ __forceinline__ int32_t merge_total(int32_t mine, int32_t (&counts)[k
   return __reduce_add_sync(kFull, lane < kMergeWarps ? counts[lane] : 0);
 }
 
+// The candidates of the pool that may be among the best, into kept / kept_code (sh.count of them):
+// those within the fewest sixteenths below the best that hold `wanted`, or, where these are many or
+// far from the best, those above an edge raised by bisection over the bits that they differ in
+// until few are left, equal scores by beam and token.
+__device__ __forceinline__ void keep_best(MergeShared& sh, const uint64_t* order, const uint32_t* code, int32_t pool,
+                                       int32_t wanted, uint64_t* kept, uint32_t* kept_code) {
+  const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int32_t most_kept = wanted < 32 ? 64 : 2 * wanted;
+  uint64_t most = 0, least = ~0ull;
+#pragma unroll 1
+  for (int32_t i = tid; i < pool; i += kMergeThreads) {
+    const uint64_t o = order[i];
+    if (o == kRisingNone) continue;
+    most = o > most ? o : most;
+    least = o < least ? o : least;
+  }
+  const uint32_t of_warp = __reduce_max_sync(kFull, most ? rising(__double2float_rn(from_rising(most))) : 0u);
+  if (lane == 0) sh.warp_top[warp] = of_warp;
+#pragma unroll 1
+  for (int32_t i = tid; i < kBuckets; i += kMergeThreads) sh.bucket[i] = 0;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  const float top = from_rising(__reduce_max_sync(kFull, lane < kMergeWarps ? sh.warp_top[lane] : 0u));
+#pragma unroll 1
+  for (int32_t i = tid; i < pool; i += kMergeThreads)
+    if (order[i] != kRisingNone) atomicAdd(&sh.bucket[bucket_of(from_rising(order[i]), top)], 1);
+  __syncthreads();
+  // which bucket holds the wanted-th: first of 32 sets of buckets, then of that set's
+  constexpr int32_t kEach = kBuckets / 32;
+  static_assert(kEach == 16, "two steps of 32 and 16");
+  int32_t upto = 0;
+#pragma unroll
+  for (int32_t i = 0; i < kEach; ++i) upto += sh.bucket[lane * kEach + i];
+#pragma unroll
+  for (int32_t d = 1; d < 32; d <<= 1) {
+    const int32_t before = __shfl_up_sync(kFull, upto, d);
+    if (lane >= d) upto += before;
+  }
+  const uint32_t sets = __ballot_sync(kFull, upto >= wanted);
+  uint64_t edge = kRisingNone + 1;  // candidates of this order, and with it of a code <= last, and above are kept
+  uint32_t last = kFull;
+  int32_t farthest = kBuckets;      // and at most this far below the best
+  if (sets) {  // else fewer than `wanted` in all: every one of them
+    const int32_t set = __ffs(sets) - 1;
+    const int32_t before_set = set > 0 ? __shfl_sync(kFull, upto, set > 0 ? set - 1 : 0) : 0;
+    int32_t within = before_set + (lane < kEach ? sh.bucket[set * kEach + lane] : 0);
+    if (lane > 0) within -= before_set;
+#pragma unroll
+    for (int32_t d = 1; d < kEach; d <<= 1) {
+      const int32_t before = __shfl_up_sync(kFull, within, d);
+      if (lane >= d) within += before;
+    }
+    const int32_t at = __ffs(__ballot_sync(kFull, lane < kEach && within >= wanted)) - 1;
+    const int32_t level0 = __shfl_sync(kFull, within, at);
+    farthest = set * kEach + at;
+    if (level0 > most_kept || farthest == kBuckets - 1) {
+      farthest = kBuckets;
+#pragma unroll 1
+      for (int32_t d = 16; d > 0; d >>= 1) {
+        const uint64_t m = __shfl_xor_sync(kFull, most, d), l = __shfl_xor_sync(kFull, least, d);
+        most = m > most ? m : most;
+        least = l < least ? l : least;
+      }
+      if (lane == 0) {
+        sh.warp_most[warp] = most;
+        sh.warp_least[warp] = least;
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int32_t w = 0; w < kMergeWarps; ++w) {
+        most = sh.warp_most[w] > most ? sh.warp_most[w] : most;
+        least = sh.warp_least[w] < least ? sh.warp_least[w] : least;
+      }
+      int32_t turn = 0, level = pool;
+      if (most > least) {
+        const int32_t top_bit = 63 - __clzll(static_cast<long long>(most ^ least));
+        uint64_t base = most & ~((2ull << top_bit) - 1ull);
+#pragma unroll 1
+        for (int32_t bit = top_bit; bit >= 0 && level > most_kept; --bit, turn ^= 1) {
+          const uint64_t trial = base | (1ull << bit);
+          int32_t mine = 0;
+#pragma unroll 1
+          for (int32_t i = tid; i < pool; i += kMergeThreads) mine += order[i] >= trial;
+          const int32_t total = merge_total(mine, sh.counts[turn]);
+          if (total >= wanted) {
+            base = trial;
+            edge = trial;
+            level = total;
+          }
+        }
+      } else {
+        edge = most;
+      }
+      if (level > most_kept) {  // equal scores: by beam and token
+        int32_t above = 0, equal = 0;
+#pragma unroll 1
+        for (int32_t i = tid; i < pool; i += kMergeThreads) {
+          above += order[i] > edge;
+          equal += order[i] == edge;
+        }
+        above = merge_total(above, sh.counts[turn]);
+        turn ^= 1;
+        equal = merge_total(equal, sh.counts[turn]);
+        turn ^= 1;
+        if (above + equal > most_kept && above < wanted) {
+          uint32_t before = kFull;  // codes up to before + 1 are kept
+#pragma unroll 1
+          for (int32_t bit = 25; bit >= 0; --bit, turn ^= 1) {
+            const uint32_t trial = before + (1u << bit);
+            int32_t mine = 0;
+#pragma unroll 1
+            for (int32_t i = tid; i < pool; i += kMergeThreads) mine += order[i] == edge && code[i] <= trial;
+            if (merge_total(mine, sh.counts[turn]) < wanted - above) before = trial;
+          }
+          last = before + 1u;
+        }
+      }
+    }
+  }
+#pragma unroll 1
+  for (int32_t i = tid; i < pool; i += kMergeThreads) {
+    const uint64_t o = order[i];
+    if (o != kRisingNone && (o > edge || (o == edge && code[i] <= last)) &&
+        (farthest == kBuckets || bucket_of(from_rising(o), top) <= farthest)) {
+      const int32_t at = atomicAdd(&sh.count, 1);
+      kept[at] = o;
+      kept_code[at] = code[i];
+    }
+  }
+  __syncthreads();
+}
+
 template <typename E>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ ScanArgs s) {
   extern __shared__ __align__(16) char dynamic[];
   __shared__ MergeShared sh;
   const SelectArgs& a = s.a;
   const int32_t pool = s.pool, beams = a.beams, shares = s.shares, wanted = a.candidates;
-  double* value = reinterpret_cast<double*>(dynamic);            // [pool]; -inf: none
-  double* kept = value + pool;                                   // [pool] the values that may be among the best
-  uint32_t* code = reinterpret_cast<uint32_t*>(kept + pool);     // [pool] beam << 20 | token
-  uint32_t* kept_code = code + pool;                             // [pool]
+  uint64_t* order = reinterpret_cast<uint64_t*>(dynamic);        // [pool] rising() of the scores
+  uint64_t* kept = order + pool;                                 // [pool] those that may be among the best
+  uint32_t* code = reinterpret_cast<uint32_t*>(kept + pool);     // [pool] beam << 20 | token, then the kept ones'
+  uint32_t* kept_code = code + pool;
   const int32_t group = blockIdx.x, row0 = group * beams;
   const int32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t of_beam = shares * wanted;
@@ -861,20 +984,23 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     const int32_t i = tid + k * kMergeThreads;
     ahead[k] = i < pool ? keys[i] : 0u;
   }
+  int32_t width = 1;
+  while (width < shares && width < 32) width <<= 1;
 #pragma unroll 1
   for (int32_t b = warp; b < beams; b += kMergeWarps) {
     const int32_t row = row0 + b;
     const float score = a.scores[row];
     const bool ended = a.finished && a.finished[row];
+    Part p{0.0, 0.0, -CUDART_INF_F, -CUDART_INF_F};
     int32_t state = 0;
     double ref = 0.0, log_sum = 0.0;
     if (isfinite(score)) {
       if (ended) {
         state = 2;
       } else {
-        Part p{0.0, 0.0, -CUDART_INF_F, -CUDART_INF_F};
+        if (lane < shares) p = s.parts[static_cast<int64_t>(row) * shares + lane];
 #pragma unroll 1
-        for (int32_t c = lane; c < shares; c += 32) {  // one for most lanes
+        for (int32_t c = lane + 32; c < shares; c += 32) {
           const Part q = s.parts[static_cast<int64_t>(row) * shares + c];
           if (q.anchor != -CUDART_INF_F) {
             const float anchor = fmaxf(p.anchor, q.anchor);
@@ -888,7 +1014,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
             p.far = far;
           }
         }
-        p = total_part(p);
+        p = total_part(p, width);
         double sum = p.sum;
         ref = p.anchor == -CUDART_INF_F ? 0.0 : static_cast<double>(p.anchor) * kLn2;
         if (p.far != -CUDART_INF_F) {
@@ -910,192 +1036,74 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       sh.log_sum[b] = log_sum;
     }
   }
-  // keep at most so many for the ordering, unless it is all there are
-  const int32_t most_kept = wanted < 32 ? 64 : 2 * wanted;
+  int32_t filled;
+#pragma unroll 1
   for (;;) {
     __syncthreads();
     // every candidate's score
-    uint64_t most = 0, least = ~0ull;
-    bool bisect = false;
     const auto place = [&](int32_t i, uint64_t key) {
       const int32_t b = i / of_beam, state = sh.state[b];
-      double v = -CUDART_INF;
-      int32_t token = 0;
+      uint64_t o = kRisingNone;
+      uint32_t token = 0;
       if (state == 2) {
         if (i == b * of_beam && a.end_token >= 0) {
-          v = sh.score[b];
+          o = rising(sh.score[b]);
           token = a.end_token;
         }
       } else if (state && key) {
-        token = static_cast<int32_t>(~static_cast<uint32_t>(key));
-        const float x = from_rising(static_cast<uint32_t>(key >> 32));
-        v = sh.score[b] + ((static_cast<double>(x) - sh.ref[b]) - sh.log_sum[b]);
-        if (!isfinite(__double2float_rn(v))) v = -CUDART_INF;
+        token = ~static_cast<uint32_t>(key);
+        const double x = from_rising(static_cast<uint32_t>(key >> 32));
+        const double v = sh.score[b] + ((x - sh.ref[b]) - sh.log_sum[b]);
+        if (isfinite(__double2float_rn(v))) o = rising(v + 0.0);
       }
-      value[i] = v;
-      code[i] = (static_cast<uint32_t>(b) << 20) | static_cast<uint32_t>(token);
-      if (v != -CUDART_INF) {
-        const uint64_t o = rising(v);
-        most = o > most ? o : most;
-        least = o < least ? o : least;
-      }
+      order[i] = o;
+      code[i] = (static_cast<uint32_t>(b) << 20) | token;
     };
 #pragma unroll
     for (int32_t k = 0; k < kMergeKeys; ++k)
       if (tid + k * kMergeThreads < pool) place(tid + k * kMergeThreads, ahead[k]);
 #pragma unroll 1
     for (int32_t i = tid + kMergeKeys * kMergeThreads; i < pool; i += kMergeThreads) place(i, keys[i]);
-    uint64_t edge = kRisingNone + 1;  // candidates of this order, and with it of a code <= last, and above are kept
-    uint32_t last = kFull;
-    int32_t farthest = kBuckets;      // and at most this far below the best
-    float top_value = 0.0f;
-    if (pool > most_kept) {
-      // the candidates within the fewest sixteenths below the best that hold `wanted`
-      const uint32_t of_warp = __reduce_max_sync(kFull, most ? rising(__double2float_rn(from_rising(most))) : 0u);
-      if (lane == 0) sh.warp_top[warp] = of_warp;
-#pragma unroll 1
-      for (int32_t i = tid; i < kBuckets; i += kMergeThreads) sh.bucket[i] = 0;
-      __syncthreads();
-      const uint32_t top = __reduce_max_sync(kFull, lane < kMergeWarps ? sh.warp_top[lane] : 0u);
-      top_value = from_rising(top);
-#pragma unroll 1
-      for (int32_t i = tid; i < pool; i += kMergeThreads)
-        if (value[i] != -CUDART_INF) atomicAdd(&sh.bucket[bucket_of(value[i], top_value)], 1);
-      __syncthreads();
-      constexpr int32_t kEach = kBuckets / 32;
-      int32_t mine = 0;
-#pragma unroll
-      for (int32_t i = 0; i < kEach; ++i) mine += sh.bucket[lane * kEach + i];
-      int32_t upto = mine;
-#pragma unroll
-      for (int32_t d = 1; d < 32; d <<= 1) {
-        const int32_t before = __shfl_up_sync(kFull, upto, d);
-        if (lane >= d) upto += before;
-      }
-      const uint32_t enough = __ballot_sync(kFull, upto >= wanted);
-      int32_t level = pool;
-      if (enough) {
-        int32_t at = (__ffs(enough) - 1) * kEach, sum = __shfl_sync(kFull, upto - mine, __ffs(enough) - 1);
-        while ((sum += sh.bucket[at]) < wanted) ++at;
-        level = sum;
-        farthest = at;
-      }
-      bisect = enough && (level > most_kept || farthest == kBuckets - 1);
-      if (bisect) farthest = kBuckets;
-    }
-    if (bisect) {  // many in one sixteenth, or far from the best: raise the edge by bisection, over
-                   // the bits that the candidates differ in, until few are left above it
-      for (int32_t d = 16; d > 0; d >>= 1) {
-        const uint64_t m = __shfl_xor_sync(kFull, most, d), l = __shfl_xor_sync(kFull, least, d);
-        most = m > most ? m : most;
-        least = l < least ? l : least;
-      }
-      if (lane == 0) {
-        sh.warp_most[warp] = most;
-        sh.warp_least[warp] = least;
-      }
-      __syncthreads();
-#pragma unroll 1
-      for (int32_t w = 0; w < kMergeWarps; ++w) {
-        most = sh.warp_most[w] > most ? sh.warp_most[w] : most;
-        least = sh.warp_least[w] < least ? sh.warp_least[w] : least;
-      }
-      int32_t turn = 0, level = pool;
-      if (most > least) {
-        const int32_t top_bit = 63 - __clzll(static_cast<long long>(most ^ least));
-        uint64_t base = most & ~((2ull << top_bit) - 1ull);
-        if (top_bit == 63) base = 0;
-#pragma unroll 1
-        for (int32_t bit = top_bit; bit >= 0 && level > most_kept; --bit, turn ^= 1) {
-          const uint64_t trial = base | (1ull << bit);
-          int32_t mine = 0;
-#pragma unroll 1
-          for (int32_t i = tid; i < pool; i += kMergeThreads) mine += rising(value[i]) >= trial;
-          const int32_t total = merge_total(mine, sh.counts[turn]);
-          if (total >= wanted) {
-            base = trial;
-            edge = trial;
-            level = total;
-          }
-        }
-      } else if (most == least) {
-        edge = most;
-      }
-      if (level > most_kept && most >= least) {  // equal scores, or few candidates: by beam and token
-        int32_t above = 0, equal = 0;
-#pragma unroll 1
-        for (int32_t i = tid; i < pool; i += kMergeThreads) {
-          const uint64_t o = rising(value[i]);
-          above += o > edge;
-          equal += o == edge;
-        }
-        above = merge_total(above, sh.counts[turn]);
-        turn ^= 1;
-        equal = merge_total(equal, sh.counts[turn]);
-        turn ^= 1;
-        if (above + equal > most_kept && above < wanted) {
-          uint32_t before = kFull;  // codes up to before + 1 are kept
-#pragma unroll 1
-          for (int32_t bit = 25; bit >= 0; --bit, turn ^= 1) {
-            const uint32_t trial = before + (1u << bit);
-            int32_t mine = 0;
-#pragma unroll 1
-            for (int32_t i = tid; i < pool; i += kMergeThreads) mine += rising(value[i]) == edge && code[i] <= trial;
-            if (merge_total(mine, sh.counts[turn]) < wanted - above) before = trial;
-          }
-          last = before + 1u;
-        }
-      }
-    }
-    if (tid == 0) sh.count = 0;
-#pragma unroll 1
-    for (int32_t b = tid; b < beams; b += kMergeThreads) sh.again[b] = 0;
-#pragma unroll 1
-    for (int32_t i = tid; i < kPoolMax / 32; i += kMergeThreads) sh.near_bits[i] = 0u;
+    if (tid < beams) sh.again[tid] = 0;
     __syncthreads();
-#pragma unroll 1
-    for (int32_t i = tid; i < pool; i += kMergeThreads) {
-      const uint64_t o = rising(value[i]);
-      if (o > kRisingNone && (o > edge || (o == edge && code[i] <= last)) &&
-          (farthest == kBuckets || bucket_of(value[i], top_value) <= farthest)) {
-        const int32_t at = atomicAdd(&sh.count, 1);
-        kept[at] = value[i];
-        kept_code[at] = code[i];
-      }
+    int32_t n = pool, at0 = 0;  // the candidates to put in order: order[at0 ..), code[at0 ..)
+    if (pool > kDirect) {
+      keep_best(sh, order, code, pool, wanted, kept, kept_code);
+      at0 = pool;
+      n = sh.count;
     }
-    __syncthreads();
-    const int32_t n = sh.count;
-    {
-      const int32_t split = split_of(n), step = kMergeThreads / split, part = tid & (split - 1);
+    // in order, by counting the better ones; several threads of a warp share an item's comparisons
+    int32_t valid = 0;
+    int32_t split = 1;
+    while (split < 32 && n * split * 2 <= kMergeThreads) split <<= 1;
+    const int32_t per_pass = kMergeThreads / split, part = tid & (split - 1);
 #pragma unroll 1
-      for (int32_t i0 = 0; i0 < n; i0 += step) {  // uniform: the shuffles below take whole warps
-        const int32_t i = i0 + tid / split;
-        int32_t rank = 0;  // and, from bit 16 on, how many of other beams are too near to tell
-        const double mine = i < n ? kept[i] : 0.0;
-        const uint32_t own = i < n ? kept_code[i] : 0u;
-        if (i < n)
+    for (int32_t i0 = 0; i0 < n; i0 += per_pass) {  // uniform: the shuffles below take whole warps
+      const int32_t i = i0 + tid / split;
+      const uint64_t mine = i < n ? order[at0 + i] : 0u;
+      const uint32_t own = i < n ? code[at0 + i] : 0u;
+      int32_t rank = 0;
+      if (mine > kRisingNone) {
+#pragma unroll 4
+        for (int32_t j = part; j < n; j += split) {
+          const uint64_t other = order[at0 + j];
+          rank += other > mine;
+          if (other == mine) rank += code[at0 + j] < own;
+        }
+      }
 #pragma unroll 1
-          for (int32_t j = part; j < n; j += split) {
-            const double ahead_by = kept[j] - mine;
-            const uint32_t other = kept_code[j];
-            rank += ahead_by > 0.0 || (ahead_by == 0.0 && other < own);
-            rank += fabs(ahead_by) <= kNear && ((other ^ own) >> 20) ? 1 << 16 : 0;
-          }
-#pragma unroll 1
-        for (int32_t d = 1; d < split; d <<= 1) rank += __shfl_xor_sync(kFull, rank, d);
-        if (i < n && part == 0) {
-          if (rank >> 16) atomicOr(&sh.near_bits[i >> 5], 1u << (i & 31));
-          rank &= 0xffff;
-          if (rank < wanted) {
-            sh.best[rank] = mine;
-            sh.best_code[rank] = own;
-          }
+      for (int32_t d = 1; d < split; d <<= 1) rank += __shfl_xor_sync(kFull, rank, d);
+      if (mine > kRisingNone && part == 0) {
+        ++valid;
+        if (rank < wanted) {
+          sh.best[rank] = mine;
+          sh.best_code[rank] = own;
         }
       }
     }
-    __syncthreads();
-    // beams whose candidates the 32-bit sums cannot order: among those that may be the best, and
-    // whatever of another beam lies as near to the last of the best
+    filled = min(merge_total(valid, sh.counts[0]), wanted);
+    // beams whose candidates the 32-bit sums cannot order: neighbours among the best, and whatever
+    // of another beam lies as near to the last of them
     bool unsure = false;
     const auto doubt = [&](uint32_t b) {
       if (sh.state[b] == 1) {
@@ -1103,20 +1111,23 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         unsure = true;
       }
     };
-    const double last_best = n >= wanted ? sh.best[wanted - 1] : -CUDART_INF;
-#pragma unroll 1
-    for (int32_t i = tid; i < n; i += kMergeThreads)
-      if (((sh.near_bits[i >> 5] >> (i & 31)) & 1u) && kept[i] >= last_best - kNear) doubt(kept_code[i] >> 20);
-    if (n >= wanted) {
+    if (tid + 1 < filled) {
+      const uint32_t p = sh.best_code[tid] >> 20, q = sh.best_code[tid + 1] >> 20;
+      if (p != q && from_rising(sh.best[tid]) - from_rising(sh.best[tid + 1]) <= kNear) {
+        doubt(p);
+        doubt(q);
+      }
+    }
+    if (filled == wanted) {
+      const uint64_t last_best = sh.best[wanted - 1];
+      const uint64_t lowest = rising(from_rising(last_best) - kNear);
       const uint32_t last_beam = sh.best_code[wanted - 1] >> 20;
 #pragma unroll 1
-      for (int32_t i = tid; i < pool; i += kMergeThreads) {
-        const uint32_t b = code[i] >> 20;
-        if (value[i] >= last_best - kNear && value[i] <= last_best && b != last_beam) {
-          doubt(b);
+      for (int32_t i = tid; i < pool; i += kMergeThreads)
+        if (order[i] >= lowest && order[i] <= last_best && (code[i] >> 20) != last_beam) {
+          doubt(code[i] >> 20);
           doubt(last_beam);
         }
-      }
     }
     if (!__syncthreads_or(unsure)) break;
 #pragma unroll 1
@@ -1129,16 +1140,15 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       }
     }
   }
-#pragma unroll 1
-  for (int32_t i = tid; i < wanted; i += kMergeThreads) {
-    const int64_t to = static_cast<int64_t>(group) * wanted + i;
+  if (tid < wanted) {
+    const int64_t to = static_cast<int64_t>(group) * wanted + tid;
     float score = -CUDART_INF_F;
     int32_t beam = -1, token = -1;
     bool ended = false;
-    if (i < min(sh.count, wanted)) {
-      score = __double2float_rn(sh.best[i]);
-      beam = static_cast<int32_t>(sh.best_code[i] >> 20);
-      token = static_cast<int32_t>(sh.best_code[i] & 0xfffffu);
+    if (tid < filled) {
+      score = __double2float_rn(from_rising(sh.best[tid]));
+      beam = static_cast<int32_t>(sh.best_code[tid] >> 20);
+      token = static_cast<int32_t>(sh.best_code[tid] & 0xfffffu);
       ended = token == a.end_token || sh.state[beam] == 2;
     }
     a.out_scores[to] = score;
