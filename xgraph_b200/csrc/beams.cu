@@ -1402,7 +1402,7 @@ __device__ __forceinline__ void copy_word_async(void* shared, const void* global
 // beam at the window's end of each last place, and a second walk of the segments every step's
 // beam, by which the tokens are picked.  So the walk is 2 * segment + segments + cluster links
 // long instead of the steps', and the rest is loads and stores side by side.
-__global__ void __launch_bounds__(kTraceThreads) trace_kernel(const __grid_constant__ TraceArgs a) {
+__global__ void __launch_bounds__(kTraceThreads, 4) trace_kernel(const __grid_constant__ TraceArgs a) {
   extern __shared__ __align__(16) uint8_t shared[];
   const int32_t beams = a.beams, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t* text = reinterpret_cast<int32_t*>(shared);        // [window][beams + 1]: rows shifted by a bank each
@@ -1412,6 +1412,7 @@ __global__ void __launch_bounds__(kTraceThreads) trace_kernel(const __grid_const
   uint8_t* enter = through + a.segments * beams;             // [segments][beams]: the beam at its end, per last place
   uint8_t* whole = enter + a.segments * beams;               // [beams]: from the window's end to before it
   uint8_t* carry = whole + kMaxBeams;                        // [beams]: the beam at the stretch's end, per last place
+  uint8_t* peers = carry + kMaxBeams;                        // [cluster][1 << log_lanes]: the windows' maps
   const int32_t group = blockIdx.x / a.cluster, rank = blockIdx.x - group * a.cluster;
   const int32_t length = a.lengths ? min(max(a.lengths[group], 0), a.steps) : a.steps;
   int32_t* out = a.out + static_cast<int64_t>(group) * beams * a.steps;
@@ -1427,20 +1428,26 @@ __global__ void __launch_bounds__(kTraceThreads) trace_kernel(const __grid_const
     const int32_t* parents = a.parents + begin * a.parent_step + group * a.parent_group + k_own;
     const int32_t* tokens = a.tokens + begin * a.token_step + group * a.token_group + k_own;
     if (has_beam) {
-      for (int32_t t = s_own; t < count; t += s_next) copy_word_async(text + t * (beams + 1) + k_own, tokens + t * a.token_step);
-      commit_async();
 #pragma unroll 8
       for (int32_t t = s_own; t < count; t += s_next) {
         const int32_t p = __ldg(parents + t * a.parent_step);
+        copy_word_async(text + t * (beams + 1) + k_own, tokens + t * a.token_step);
         maps[t * beams + k_own] = p >= 0 && p < beams ? static_cast<uint8_t>(p) : kNoBeam;
       }
+      commit_async();
     }
     __syncthreads();
-    for (int32_t s = s_own; s < segments && has_beam; s += s_next) {
+    // two segments at a time, so that one's load is in flight while the other's is waited for
+    for (int32_t s = s_own; s < segments && has_beam; s += 2 * s_next) {
       const int32_t t0 = s * a.segment, t1 = min(t0 + a.segment, count);
-      int32_t at = k_own;
-      for (int32_t t = t1 - 1; t >= t0 && at != kNoBeam; --t) at = maps[t * beams + at];
+      const int32_t u0 = (s + s_next) * a.segment, u1 = min(u0 + a.segment, count);
+      int32_t at = k_own, to = k_own;
+      for (int32_t t = t1 - 1, u = u1 - 1; t >= t0 || u >= u0; --t, --u) {
+        if (t >= t0 && at != kNoBeam) at = maps[t * beams + at];
+        if (u >= u0 && to != kNoBeam) to = maps[u * beams + to];
+      }
       through[s * beams + k_own] = static_cast<uint8_t>(at);
+      if (u0 < count) through[(s + s_next) * beams + k_own] = static_cast<uint8_t>(to);
     }
     __syncthreads();
     if (tid < beams) {
@@ -1449,11 +1456,15 @@ __global__ void __launch_bounds__(kTraceThreads) trace_kernel(const __grid_const
       whole[tid] = static_cast<uint8_t>(at);
     }
     cluster_sync();
+    // the windows' maps of the whole stretch, fetched side by side
+    for (int32_t i = tid; i < a.cluster << a.log_lanes; i += kTraceThreads)
+      if (has_beam) peers[i] = peer_byte(whole + k_own, i >> a.log_lanes);
+    __syncthreads();
     if (tid < beams) {
       int32_t at = carry[tid];
-      for (int32_t r = 0; r < rank && at != kNoBeam; ++r) at = peer_byte(whole + at, r);
+      for (int32_t r = 0; r < rank && at != kNoBeam; ++r) at = peers[(r << a.log_lanes) + at];
       int32_t before = at;  // and on to before the stretch
-      for (int32_t r = rank; r < a.cluster && before != kNoBeam && stop > stretch; ++r) before = peer_byte(whole + before, r);
+      for (int32_t r = rank; r < a.cluster && before != kNoBeam; ++r) before = peers[(r << a.log_lanes) + before];
       carry[tid] = static_cast<uint8_t>(before);
       for (int32_t s = segments - 1; s >= 0; --s) {
         enter[s * beams + tid] = static_cast<uint8_t>(at);
@@ -1461,18 +1472,27 @@ __global__ void __launch_bounds__(kTraceThreads) trace_kernel(const __grid_const
       }
     }
     __syncthreads();
-    for (int32_t s = s_own; s < segments && has_beam; s += s_next) {
+    uint8_t* own_way = way + k_own * a.way_stride;
+    for (int32_t s = s_own; s < segments && has_beam; s += 2 * s_next) {
       const int32_t t0 = s * a.segment, t1 = min(t0 + a.segment, count);
-      int32_t at = enter[s * beams + k_own];
-      for (int32_t t = t1 - 1; t >= t0; --t) {
-        way[k_own * a.way_stride + t] = static_cast<uint8_t>(at);
-        if (at != kNoBeam) at = maps[t * beams + at];
+      const int32_t u0 = (s + s_next) * a.segment, u1 = min(u0 + a.segment, count);
+      int32_t at = enter[s * beams + k_own], to = u0 < count ? enter[(s + s_next) * beams + k_own] : kNoBeam;
+      for (int32_t t = t1 - 1, u = u1 - 1; t >= t0 || u >= u0; --t, --u) {
+        if (t >= t0) {
+          own_way[t] = static_cast<uint8_t>(at);
+          if (at != kNoBeam) at = maps[t * beams + at];
+        }
+        if (u >= u0) {
+          own_way[u] = static_cast<uint8_t>(to);
+          if (to != kNoBeam) to = maps[u * beams + to];
+        }
       }
     }
     wait_async<0>();
     cluster_sync();  // the ways and texts are there, and the window's map has been read by the others
     for (int32_t k = warp; k < beams; k += kTraceWarps) {
       int32_t* to = out + static_cast<int64_t>(k) * a.steps + begin;
+#pragma unroll 8
       for (int32_t t = lane; t < count; t += 32) {
         const int32_t at = way[k * a.way_stride + t];
         to[t] = at == kNoBeam ? a.pad : text[t * (beams + 1) + at];
@@ -1873,7 +1893,7 @@ extern "C" XG_API int xg_beam_sequences(const int32_t* tokens, int64_t token_ste
   while (a.segment * a.segment < a.window) a.segment *= 2;
   a.segments = (a.window + a.segment - 1) / a.segment;
   const int32_t bytes = a.window * (beams + 1) * 4 + a.window * beams + a.way_stride * beams + 2 * a.segments * beams +
-                        2 * kMaxBeams;
+                        (2 + a.cluster) * kMaxBeams;
   static std::atomic<bool> allowed[kDevices];
   if (int rc = allow_shared(reinterpret_cast<const void*>(trace_kernel), 2 * kTraceBytes, allowed)) return rc;
   cudaLaunchConfig_t config{};
