@@ -151,7 +151,7 @@ def test_layouts_of_tensors():
     with pytest.raises(ValueError, match="share memory"):
         _row_tensors([a, b, a], None, cpu)
     for tensor, dim in ((torch.zeros(()), None), (torch.zeros((1,) * 6), None), (a, 0), (a, 3), (a, -3),
-                        (torch.zeros((4, 4)).to_sparse(), None)):
+                        (torch.zeros((4, 4)).to_sparse(), None), (torch.zeros((4, 4), requires_grad=True), None)):
         with pytest.raises((ValueError, RuntimeError)):
             _layout(tensor, dim, cpu)
 

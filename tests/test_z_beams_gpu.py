@@ -121,6 +121,39 @@ def test_equal_logits_go_to_the_lowest_token(dtype):
     check(torch.zeros_like(logits), scores, 128, renormalize=False, mask=make_mask(8, 20011, 4, (0.9,)))
 
 
+@pytest.mark.parametrize("dtype,vocab", [("float32", 140001), ("bfloat16", 270000)])
+def test_a_row_of_several_rounds(dtype, vocab):
+    """64 beams of 128 candidates leave one CTA to a row, which takes its best out in rounds:
+    ties over all of them, and rows whose tokens lie in one."""
+    import torch
+
+    logits = torch.zeros((64, vocab), dtype=getattr(torch, dtype), device="cuda")
+    logits[8:16] = make(dtype, 8, vocab, 3)
+    logits[16:24, : vocab // 2] = -4.0
+    logits[24:32, vocab - 9:] = 3.0
+    logits[32:40, :5] = 2.0
+    bits = np.ones((64, (vocab + 31) // 32 * 32), dtype=bool)
+    bits[40:48, : vocab - 700] = False
+    bits[48:56, 300:] = False
+    bits[56] = False
+    bits[57:60, 5:vocab - 5] = False
+    mask = torch.from_numpy(np.packbits(bits, axis=1, bitorder="little").view(np.int32)).cuda()
+    scores = random_scores(1, 64, 3)
+    check(logits, scores, 128, mask=mask)
+    check(logits, scores, 128, mask=mask, renormalize=False)
+    check(logits, torch.zeros_like(scores), 128)
+
+
+def test_scores_of_zero_tie_whatever_their_sign():
+    import torch
+
+    scores = torch.tensor([[-0.0, 0.0, -0.0, 0.0]], device="cuda")
+    finished = torch.tensor([[True, False, True, True]], device="cuda")
+    logits = torch.full((4, 7), -float("inf"), device="cuda")
+    logits[:, 3] = 1.5
+    check(logits, scores, 4, finished=finished, end_token=5)
+
+
 @pytest.mark.parametrize("order", ["rising", "falling"])
 def test_sorted_logits(order):
     import torch
@@ -274,6 +307,56 @@ def test_select_in_a_graph_and_on_another_stream():
                 assert torch.equal(a, b)
 
 
+def test_select_refusals():
+    import torch
+
+    from xgraph_b200.beams import beam_select
+
+    logits, scores = make("float32", 8, 100, 3), random_scores(2, 4, 3)
+    mask, finished = make_mask(8, 100, 3), torch.zeros((2, 4), dtype=torch.bool, device="cuda")
+    beam_select(logits, scores, mask=mask, finished=finished, end_token=3)
+    for change, message in [
+        (dict(logits=logits.double()), "float32, bfloat16 or float16"), (dict(logits=logits[0]), "2-D"),
+        (dict(logits=logits.t()), "contiguous row|row per beam"), (dict(logits=logits[:7]), "one row per beam"),
+        (dict(logits=logits[:1].expand(8, -1)), "overlap"), (dict(scores=scores[0]), "groups, beams"),
+        (dict(scores=scores.half()), "float32"), (dict(scores=scores.cpu()), "on cuda"),
+        (dict(scores=scores.t().contiguous().t()), "contiguous"), (dict(mask=mask.long()), "int32"),
+        (dict(mask=mask[:, :3]), "words"), (dict(mask=mask[:7]), "rows"),
+        (dict(mask=mask[:1].expand(8, -1)), "overlap"), (dict(mask=mask.t().contiguous().t()), "contiguous row"),
+        (dict(finished=finished.int()), "bool"), (dict(finished=finished[:, :3]), "shape"),
+        (dict(end_token=None), "end_token"), (dict(end_token=100), "end_token"), (dict(end_token=-1), "end_token"),
+        (dict(candidates=0), "candidates"), (dict(candidates=129), "candidates"), (dict(vocab=101), "vocab"),
+        (dict(vocab=0), "vocab"), (dict(scores=torch.zeros((8, 0), device="cuda"), logits=logits[:0]), "beams"),
+    ]:
+        call = {"logits": logits, "scores": scores, "mask": mask, "finished": finished, "end_token": 3, **change}
+        if "scores" in change and change["scores"].numel() == 0:
+            call.update(mask=None, finished=None, end_token=None)
+        with pytest.raises(ValueError, match=message):
+            beam_select(call.pop("logits"), call.pop("scores"), **call)
+    empty = beam_select(logits[:0], scores[:0], candidates=5)
+    assert empty.scores.shape == (0, 5) and empty.finished.shape == (0, 5)
+
+
+def test_overlapping_calls_on_two_streams():
+    """Calls in flight together keep their own workspaces."""
+    import torch
+
+    from xgraph_b200.beams import beam_select
+
+    inputs = [(make("bfloat16", 32, 60000, k), random_scores(4, 8, k)) for k in range(2)]
+    want = [beam_select(*i, candidates=16) for i in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for k, stream in enumerate(streams):
+            got[k].append(beam_select(*inputs[k], candidates=16, stream=stream.cuda_stream))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for result in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(result, want[k]))
+
+
 # ---------------------------------------------------------------------------------------
 
 def parents_of(groups, beams, seed, shape=()):
@@ -379,6 +462,38 @@ def test_reorder_named_rows():
     check_reorder([filled((40, 9), torch.int32)], parents_of(3, 8, 6), rows=rows)
 
 
+def test_reorder_refusals():
+    import torch
+
+    from xgraph_b200.beams import beam_reorder
+
+    beams = torch.zeros((2, 4), dtype=torch.int32, device="cuda")
+    cache, lengths = filled((8, 3, 5), torch.float32), torch.zeros(2, dtype=torch.int32, device="cuda")
+    beam_reorder([], beams)
+    for args, options, message in [
+        (([cache, cache], beams), {}, "share memory"), (([cache, cache[:, 1:]], beams), dict(rows=beams), "share memory"),
+        (([cache[:7]], beams), {}, "8 rows"), (([cache, filled((9, 2), torch.int32)], beams), {}, "same number of rows"),
+        (([cache.cpu()], beams), {}, "on cuda"), (([cache], beams.cpu()), {}, "GPU"), (([cache], beams.long()), {}, "int32"),
+        (([cache], beams), dict(dim=1), "lengths"), (([cache], beams), dict(lengths=lengths), "dim"),
+        (([cache], beams), dict(lengths=lengths, dim=3), "dim"), (([cache], beams), dict(lengths=lengths, dim=0), "dim"),
+        (([cache], beams), dict(lengths=lengths, dim=[1, 1]), "one entry per tensor"),
+        (([cache], beams), dict(lengths=lengths[:1], dim=1), "shape"), (([cache], beams), dict(rows=beams[:1]), "shape"),
+        (([cache[:1].expand(8, -1, -1)], beams), {}, "overlap"), (([None], beams), {}, "torch tensors"),
+        (([cache.clone().requires_grad_()], beams), {}, "gradients"),
+        (([filled((8, 3, 4, 5, 6), torch.float32)[:, ::2, ::2, ::2, ::2]], beams), {}, "two places"),
+    ]:
+        with pytest.raises(ValueError, match=message):
+            beam_reorder(*args, **options)
+
+
+def test_reorder_interleaved_halves():
+    """Two views of one buffer that share no element are two tensors."""
+    import torch
+
+    both = filled((8, 2, 6, 16), torch.bfloat16)
+    check_reorder([both[:, 0], both[:, 1]], parents_of(2, 4, 3), lengths=[3, 6], dim=1)
+
+
 def test_reorder_a_cache_past_32_bits():
     """Rows more than 2^31 bytes from the tensor's start."""
     import torch
@@ -431,6 +546,24 @@ def test_sequences(beams, steps):
         given = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
         got = beam_sequences(torch.from_numpy(tokens).cuda(), torch.from_numpy(parents).cuda(), lengths=given, pad_token=-7)
         np.testing.assert_array_equal(got.cpu().numpy(), ref.sequences(tokens, parents, lengths=lengths, pad=-7))
+
+
+def test_sequences_refusals():
+    import torch
+
+    from xgraph_b200.beams import beam_sequences
+
+    trace = torch.zeros((6, 2, 4), dtype=torch.int32, device="cuda")
+    for args, options, message in [
+        ((trace.long(), trace), {}, "int32"), ((trace, trace[:5]), {}, "same shape"), ((trace[0], trace[0]), {}, "3-D"),
+        ((trace, trace.transpose(1, 2).contiguous().transpose(1, 2)), {}, "unit stride"),
+        ((trace, trace), dict(lengths=torch.zeros(3, dtype=torch.int32, device="cuda")), "shape"),
+        ((trace, trace), dict(pad_token=1 << 31), "int32"),
+        ((torch.zeros((2, 2, 65), dtype=torch.int32, device="cuda"),) * 2, {}, "1 to 64 beams"),
+    ]:
+        with pytest.raises(ValueError, match=message):
+            beam_sequences(*args, **options)
+    assert beam_sequences(trace[:, :0], trace[:, :0]).shape == (0, 4, 6)
 
 
 def test_sequences_longer_than_a_window_and_strided():

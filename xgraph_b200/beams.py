@@ -249,7 +249,7 @@ def _row_tensors(tensors, dim, device) -> tuple[bytes, int]:
     shape, stride, dtype = first.shape, first.stride(), first.dtype
     if not isinstance(dim, list) and all(
             [isinstance(t, kind) and t.shape == shape and t.dtype == dtype and t.stride() == stride
-             and t.device == device for t in tensors]):
+             and t.device == device and not t.requires_grad for t in tensors]):
         layout, size, dense = _layout(first, dim, device)  # one layout for all, as a model's layers have
         places = [t.data_ptr() for t in tensors]
         if len(places) > 1 and size:
@@ -278,8 +278,8 @@ def _layout(tensor, dim, device) -> tuple[bytes, int, bool]:
     size = tensor.element_size()
     if size not in (1, 2, 4, 8, 16) or tensor.layout != _torch.strided:
         raise ValueError(f"{tensor.dtype} tensors cannot be reordered")
-    if tensor.is_neg() or tensor.is_conj():
-        raise ValueError("lazily negated or conjugated tensors cannot be reordered")
+    if tensor.is_neg() or tensor.is_conj() or tensor.requires_grad:
+        raise ValueError("tensors that are lazily negated or conjugated, or need gradients, cannot be reordered")
     count = tensor.dim() - 1
     position = -1
     if dim is not None:
@@ -297,15 +297,16 @@ def _layout(tensor, dim, device) -> tuple[bytes, int, bool]:
 
 
 def _check_apart(spans):
-    """Refuse tensors that share memory: the same place twice, or overlapping dense ones."""
-    end, start, dense = -1, -1, False
-    for at, size, whole in sorted(spans):
-        if size and (at == start or (at < end and whole and dense)):
+    """Refuse tensors that share memory: two that begin at one place, or one that begins inside
+    another without gaps.  (Interleaved ones, whose gaps hold each other, are apart.)"""
+    filled, start = -1, -1  # the end of the dense tensors so far, and the last one's begin
+    for at, size, dense in sorted(spans):
+        if size and (at == start or at < filled):
             raise ValueError("the tensors share memory")
         if size:
             start = at
-            if at + size > end:
-                end, dense = at + size, whole
+            if dense:
+                filled = max(filled, at + size)
 
 
 def beam_sequences(tokens, beams, *, lengths=None, pad_token: int = -1, stream: int = 0):

@@ -1047,7 +1047,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       uint32_t token = 0;
       if (state == 2) {
         if (i == b * of_beam && a.end_token >= 0) {
-          o = rising(sh.score[b]);
+          o = rising(sh.score[b] + 0.0);
           token = a.end_token;
         }
       } else if (state && key) {
