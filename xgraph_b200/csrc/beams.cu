@@ -84,6 +84,7 @@ struct F32 {
   static constexpr uint32_t kNegInf = 0xff800000u;
   __device__ static float at(const uint4& v, int k) { return __uint_as_float((&v.x)[k]); }
   __device__ static float one(const char* p) { return *reinterpret_cast<const float*>(p); }
+  __device__ static uint32_t raw(const char* p) { return *reinterpret_cast<const uint32_t*>(p); }
   __device__ static void put(uint4& v, int k, const char* p) { (&v.x)[k] = *reinterpret_cast<const uint32_t*>(p); }
   __device__ static float top(const uint4 (&v)[kVecs]) {
     float m = __uint_as_float(v[0].x);
@@ -105,6 +106,7 @@ template <uint32_t NEG_INF>
 struct Half {  // either 16-bit type
   static constexpr int kPer = 8, kBytes = 2;
   static constexpr uint32_t kNegInf = NEG_INF | (NEG_INF << 16);
+  __device__ static uint32_t raw(const char* p) { return *reinterpret_cast<const uint16_t*>(p); }
   __device__ static void put(uint4& v, int k, const char* p) {
     uint32_t& w = (&v.x)[k >> 1];
     const uint32_t b = *reinterpret_cast<const uint16_t*>(p);
@@ -773,9 +775,10 @@ struct MergeShared {
   double score[kMaxBeams];
   int32_t state[kMaxBeams];    // 0 offers nothing, 1 candidates, 2 ended, 3 candidates, 64-bit sum
   int32_t again[kMaxBeams];
+  int32_t like[kMaxBeams];     // the first beam known to have the same row: what holds of its sum holds of this one's
   uint64_t best[kMaxCandidates];  // rising() of the best scores, and their codes
   uint32_t best_code[kMaxCandidates];
-  double warp_sum[kMergeWarps];
+  double warp_sum[kMergeWarps], table[64];
   unsigned long long warp_most[kMergeWarps], warp_least[kMergeWarps];
   uint32_t warp_top[kMergeWarps];
   int32_t counts[2][kMergeWarps];
@@ -783,16 +786,41 @@ struct MergeShared {
   int32_t count;
 };
 
-// Sum over N_r of exp(x - ref) in 64 bits, by the whole CTA.
+// exp(x) in 64 bits for x from -700 to 700, smaller ones 0: with k the whole number nearest
+// 64 x / ln 2 and r the rest, exp(x) = 2^(k / 64) exp(r), where 2^(j / 64) for j = 0 .. 63 comes
+// from a table, exp(r) for |r| <= ln 2 / 128 from its series (the next term is below 2^-54) and the
+// whole power of two is added to the exponent (the table-driven method of Tang, ACM TOMS 1989).
+// A fifth of the 64-bit operations of a general exp, which is what bounds a row's sum.
+constexpr double kLn2Part = 0.693147180559945309417 / 64.0;
+constexpr double kLn2PartHi = static_cast<double>(static_cast<float>(kLn2Part));  // 24 bits: its product with k is exact
+constexpr double kLn2PartLo = kLn2Part - kLn2PartHi;
+__device__ __forceinline__ double table_exp(double x, const double* table) {
+  if (x < -700.0) return 0.0;
+  const double k = rint(x * (64.0 / 0.693147180559945309417));
+  const double r = fma(-k, kLn2PartLo, fma(-k, kLn2PartHi, x));
+  double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  const int32_t n = static_cast<int32_t>(k);
+  const double e = p * table[n & 63];
+  return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+}
+
+// Sum over N_r of exp(x - ref) in 64 bits, by the whole CTA; ref is near the row's maximum.
 template <typename E>
-__device__ __noinline__ double row_sum(const SelectArgs& a, int32_t row, double ref, double (&scratch)[kMergeWarps]) {
+__device__ __noinline__ double row_sum(const SelectArgs& a, int32_t row, double ref, double (&scratch)[kMergeWarps],
+                                       double (&table)[64]) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x / 64.0);
+  __syncthreads();
   const char* logits = a.logits + static_cast<int64_t>(row) * a.row_stride * E::kBytes;
   const RowMask mask = a.renormalize ? row_mask(a.masks, row) : RowMask{nullptr, nullptr};
   double sum = 0.0;
-#pragma unroll 1
+#pragma unroll 4
   for (int32_t t = threadIdx.x; t < a.vocab; t += kMergeThreads) {
-    if (!mask.all() && !((mask.word(t >> 5) >> (t & 31)) & 1u)) continue;
-    sum += exp(static_cast<double>(E::one(logits + static_cast<int64_t>(t) * E::kBytes)) - ref);
+    const double x = E::one(logits + static_cast<int64_t>(t) * E::kBytes);
+    if (mask.all() || ((mask.word(t >> 5) >> (t & 31)) & 1u)) sum += table_exp(x - ref, table);
   }
 #pragma unroll
   for (int32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
@@ -803,6 +831,33 @@ __device__ __noinline__ double row_sum(const SelectArgs& a, int32_t row, double 
   for (int32_t w = 0; w < kMergeWarps; ++w) sum += scratch[w];
   __syncthreads();
   return sum;
+}
+
+// Two rows hold the same logits and masks bit for bit, so that their sums are equal.
+template <typename E>
+__device__ __noinline__ bool rows_alike(const SelectArgs& a, int32_t row, int32_t other) {
+  const char* p = a.logits + static_cast<int64_t>(row) * a.row_stride * E::kBytes;
+  const char* q = a.logits + static_cast<int64_t>(other) * a.row_stride * E::kBytes;
+  bool differ = false;
+  int32_t t = 0;
+  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0) {
+#pragma unroll 8
+    for (int32_t v = threadIdx.x; v < a.vocab / E::kPer; v += kMergeThreads) {
+      const uint4 x = reinterpret_cast<const uint4*>(p)[v], y = reinterpret_cast<const uint4*>(q)[v];
+      differ |= x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w;
+    }
+    t = a.vocab / E::kPer * E::kPer;
+  }
+#pragma unroll 4
+  for (t += threadIdx.x; t < a.vocab; t += kMergeThreads)
+    differ |= E::raw(p + static_cast<int64_t>(t) * E::kBytes) != E::raw(q + static_cast<int64_t>(t) * E::kBytes);
+  if (a.renormalize) {
+    const RowMask m = row_mask(a.masks, row), n = row_mask(a.masks, other);
+    if (!m.all() || !n.all())
+      for (int32_t w = threadIdx.x; w < (a.vocab + 31) / 32; w += kMergeThreads)
+        differ |= (m.all() ? kFull : m.word(w)) != (n.all() ? kFull : n.word(w));
+  }
+  return !__syncthreads_or(differ);
 }
 
 // Doubles as unsigned integers of the same order.
@@ -1034,8 +1089,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       sh.state[b] = state;
       sh.ref[b] = ref;
       sh.log_sum[b] = log_sum;
+      sh.like[b] = b;
     }
   }
+  bool compared = false;
   int32_t filled;
 #pragma unroll 1
   for (;;) {
@@ -1113,7 +1170,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     };
     if (tid + 1 < filled) {
       const uint32_t p = sh.best_code[tid] >> 20, q = sh.best_code[tid + 1] >> 20;
-      if (p != q && from_rising(sh.best[tid]) - from_rising(sh.best[tid + 1]) <= kNear) {
+      if (sh.like[p] != sh.like[q] && from_rising(sh.best[tid]) - from_rising(sh.best[tid + 1]) <= kNear) {
         doubt(p);
         doubt(q);
       }
@@ -1124,20 +1181,39 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
       const uint32_t last_beam = sh.best_code[wanted - 1] >> 20;
 #pragma unroll 1
       for (int32_t i = tid; i < pool; i += kMergeThreads)
-        if (order[i] >= lowest && order[i] <= last_best && (code[i] >> 20) != last_beam) {
+        if (order[i] >= lowest && order[i] <= last_best && sh.like[code[i] >> 20] != sh.like[last_beam]) {
           doubt(code[i] >> 20);
           doubt(last_beam);
         }
     }
     if (!__syncthreads_or(unsure)) break;
+    if (!compared) {
+      // equal rows (a padded batch's, a beam given twice) have equal sums: nothing to tell apart
+      compared = true;
+      bool found = false;
+#pragma unroll 1
+      for (int32_t b = 1; b < beams; ++b)
+#pragma unroll 1
+        for (int32_t c = 0; c < b; ++c)
+          if (sh.again[b] && sh.again[c] && sh.like[b] == b && sh.like[c] == c && sh.log_sum[b] == sh.log_sum[c] &&
+              sh.ref[b] == sh.ref[c] && rows_alike<E>(a, row0 + b, row0 + c)) {
+            __syncthreads();
+            if (tid == 0) sh.like[b] = c;
+            __syncthreads();
+            found = true;
+          }
+      if (found) continue;
+    }
 #pragma unroll 1
     for (int32_t b = 0; b < beams; ++b) {  // at most once for each beam
-      if (!sh.again[b]) continue;
-      const double sum = row_sum<E>(a, row0 + b, sh.ref[b], sh.warp_sum);
-      if (tid == 0) {
-        sh.log_sum[b] = log(sum);
-        sh.state[b] = 3;
+      if (!sh.again[b] || sh.state[b] != 1) continue;
+      const int32_t first = sh.like[b];
+      const double sum = row_sum<E>(a, row0 + first, sh.ref[first], sh.warp_sum, sh.table);
+      if (tid < beams && sh.like[tid] == first && sh.state[tid] == 1) {
+        sh.log_sum[tid] = log(sum);
+        sh.state[tid] = 3;
       }
+      __syncthreads();
     }
   }
   if (tid < wanted) {
