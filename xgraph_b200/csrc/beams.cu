@@ -254,6 +254,23 @@ __device__ __forceinline__ int32_t block_total(int32_t mine, int32_t (&counts)[k
   return total;
 }
 
+__device__ __forceinline__ uint32_t block_most(uint32_t mine, int32_t (&counts)[kScanWarps]) {
+  const uint32_t of_warp = __reduce_max_sync(kFull, mine);
+  __syncthreads();  // whoever used the counts before has read them
+  if ((threadIdx.x & 31) == 0) counts[threadIdx.x >> 5] = static_cast<int32_t>(of_warp);
+  __syncthreads();
+  uint32_t most = 0;
+#pragma unroll
+  for (int32_t w = 0; w < kScanWarps; ++w) most = max(most, static_cast<uint32_t>(counts[w]));
+  return most;
+}
+
+// Where a bisection between two orders starts: the bits that both have, the others 0 (all of them,
+// if the two are equal).
+__device__ __forceinline__ uint32_t above_common(uint32_t bound, uint32_t most) {
+  return bound == most ? most : most & ~((2u << (31 - __clz(bound ^ most))) - 1u);
+}
+
 // At most kRankMost of the n keys in sh.pushed, `wanted` best among them: the keys are bisected
 // until few are above the edge.  Returns how many are left.
 __device__ __noinline__ int32_t fewer_keys(ScanShared& sh, int32_t n, int32_t wanted) {
@@ -317,7 +334,7 @@ __device__ __forceinline__ int32_t vector_token(int32_t entry, int32_t j, int32_
 // the entries above it are taken and, of those at it, the ones of the earliest steps that hold
 // `wanted` together: a later step's equal tokens come after theirs.  That is fewer than
 // 2 * wanted + kScanThreads <= kListCap entries.  Returns the bound.
-__device__ __noinline__ uint32_t list_crowded(ScanShared& sh, int32_t steps, int32_t wanted) {
+__device__ __noinline__ uint32_t list_crowded(ScanShared& sh, uint32_t bound, int32_t steps, int32_t wanted) {
   const int32_t tid = threadIdx.x;
   int32_t turn = 0;
   const auto count_if = [&](auto pick) {
@@ -327,9 +344,12 @@ __device__ __noinline__ uint32_t list_crowded(ScanShared& sh, int32_t steps, int
     turn ^= 1;
     return block_total(mine, sh.counts[turn]);
   };
-  uint32_t edge = 0;
   int32_t level = 0x7fffffff, last = kRound;  // entries at the edge are taken up to step `last`
-  for (int32_t bit = 31; bit >= 0 && level > kRankMost; --bit) {
+  uint32_t most = 0;
+  for (int32_t step = 0; step < steps; ++step) most = max(most, sh.tops[step][tid]);
+  most = block_most(most, sh.counts[0]);
+  uint32_t edge = above_common(bound, most);
+  for (int32_t bit = 31 - __clz(bound ^ most); bit >= 0 && level > kRankMost; --bit) {
     const uint32_t trial = edge | (1u << bit);
     const int32_t total = count_if([=](uint32_t o, int32_t) { return o >= trial; });
     if (total >= wanted) {
@@ -362,7 +382,8 @@ __device__ __noinline__ uint32_t list_crowded(ScanShared& sh, int32_t steps, int
 // most kRankMost do, and where equal logits do not let it, the lowest tokens are taken.  Their
 // keys, `wanted` to kRankMost, follow the `held` ones in sh.pushed.
 template <typename E>
-__device__ __noinline__ void push_crowded(ScanShared& sh, int32_t vectors, int32_t first, int32_t held, int32_t wanted) {
+__device__ __noinline__ void push_crowded(ScanShared& sh, uint32_t bound, int32_t vectors, int32_t first, int32_t held,
+                                          int32_t wanted) {
   constexpr int32_t kPer = E::kPer;
   const int32_t tid = threadIdx.x;
   int32_t turn = 0;
@@ -370,17 +391,25 @@ __device__ __noinline__ void push_crowded(ScanShared& sh, int32_t vectors, int32
     int32_t mine = 0;
 #pragma unroll 1
     for (int32_t i = tid; i < vectors; i += kScanThreads) {
-      const char* v = reinterpret_cast<const char*>(sh.ring + i);
+      const uint4 v = sh.ring[i];
       const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
-#pragma unroll 2
-      for (int32_t k = 0; k < kPer; ++k) mine += pick(rising(E::one(v + k * E::kBytes) + 0.0f), t0 + k);
+#pragma unroll
+      for (int32_t k = 0; k < kPer; ++k) mine += pick(rising(E::at(v, k) + 0.0f), t0 + k);
     }
     turn ^= 1;
     return block_total(mine, sh.counts[turn]);
   };
-  uint32_t edge = 0;
   int32_t level = 0x7fffffff, last = 0x7fffffff;  // of the tokens equal to the edge, those up to `last`
-  for (int32_t bit = 31; bit >= 0 && level > kRankMost; --bit) {
+  uint32_t most = 0;
+#pragma unroll 1
+  for (int32_t i = tid; i < vectors; i += kScanThreads) {
+    const uint4 v = sh.ring[i];
+#pragma unroll
+    for (int32_t k = 0; k < kPer; ++k) most = max(most, rising(E::at(v, k) + 0.0f));
+  }
+  most = block_most(most, sh.counts[0]);
+  uint32_t edge = above_common(bound, most);
+  for (int32_t bit = 31 - __clz(bound ^ most); bit >= 0 && level > kRankMost; --bit) {
     const uint32_t trial = edge | (1u << bit);
     const int32_t total = count_if([=](uint32_t o, int32_t) { return o >= trial; });
     if (total >= wanted) {
@@ -390,8 +419,19 @@ __device__ __noinline__ void push_crowded(ScanShared& sh, int32_t vectors, int32
   }
   if (level > kRankMost) {
     const int32_t above = count_if([=](uint32_t o, int32_t) { return o > edge; });
-    last = -1;
-    for (int32_t bit = 20; bit >= 0; --bit) {
+    // the lowest tokens at the edge, by bisection over the listed steps' tokens
+    int32_t low = 0x7fffffff, high = 0;
+#pragma unroll 1
+    for (int32_t i = tid; i < vectors; i += kScanThreads) {
+      const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
+      low = min(low, t0);
+      high = max(high, t0 + kPer);
+    }
+    low = static_cast<int32_t>(0x7fffffffu - block_most(0x7fffffffu - static_cast<uint32_t>(low), sh.counts[0]));
+    high = static_cast<int32_t>(block_most(static_cast<uint32_t>(high), sh.counts[1]));
+    turn = 1;
+    last = low - 1;  // too few up to here
+    for (int32_t bit = 31 - __clz(high - low + 1); bit >= 0; --bit) {
       const int32_t trial = last + (1 << bit);
       if (count_if([=](uint32_t o, int32_t t) { return o == edge && t <= trial; }) < wanted - above) last = trial;
     }
@@ -403,11 +443,11 @@ __device__ __noinline__ void push_crowded(ScanShared& sh, int32_t vectors, int32
   __syncthreads();
 #pragma unroll 1
   for (int32_t i = tid; i < vectors; i += kScanThreads) {
-    const char* v = reinterpret_cast<const char*>(sh.ring + i);
+    const uint4 v = sh.ring[i];
     const int32_t t0 = vector_token<E>(sh.list[i / kVecs], i % kVecs, first);
-#pragma unroll 1
+#pragma unroll
     for (int32_t k = 0; k < kPer; ++k) {
-      const uint32_t o = rising(E::one(v + k * E::kBytes) + 0.0f);
+      const uint32_t o = rising(E::at(v, k) + 0.0f);
       if (o >= edge && (o > edge || t0 + k <= last)) {
         const int32_t n = atomicAdd(&sh.count, 1);
         if (n < kPushCap) sh.pushed[n] = make_key(o, t0 + k);
@@ -705,7 +745,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
       }
     }
     __syncthreads();
-    if (sh.listed > kListCap) bound = max(bound, list_crowded(sh, steps, wanted));
+    if (sh.listed > kListCap) bound = max(bound, list_crowded(sh, bound, steps, wanted));
     const int32_t vectors = min(sh.listed, kListCap) * kVecs;
     if (tid < held) sh.pushed[tid] = sh.few[tid];  // the table's memory: every entry has been read
     if (tid == 0) sh.count = held;
@@ -734,7 +774,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
         over |= n >= kPushCap;
       }
     }
-    if (__syncthreads_or(over)) push_crowded<E>(sh, vectors, first, held, wanted);
+    if (__syncthreads_or(over)) push_crowded<E>(sh, bound, vectors, first, held, wanted);
     held = best_of(sh, min(sh.count, kPushCap), wanted);
   }
   if (!scans) return;  // a share past the row's end
@@ -786,7 +826,7 @@ struct MergeShared {
   int32_t count;
 };
 
-// exp(x) in 64 bits for x from -700 to 700, smaller ones 0: with k the whole number nearest
+// exp(x) in 64 bits for x up to 700 (below -700, where a sum of 1 or more does not see it, exp(-700)): with k the whole number nearest
 // 64 x / ln 2 and r the rest, exp(x) = 2^(k / 64) exp(r), where 2^(j / 64) for j = 0 .. 63 comes
 // from a table, exp(r) for |r| <= ln 2 / 128 from its series (the next term is below 2^-54) and the
 // whole power of two is added to the exponent (the table-driven method of Tang, ACM TOMS 1989).
@@ -795,7 +835,7 @@ constexpr double kLn2Part = 0.693147180559945309417 / 64.0;
 constexpr double kLn2PartHi = static_cast<double>(static_cast<float>(kLn2Part));  // 24 bits: its product with k is exact
 constexpr double kLn2PartLo = kLn2Part - kLn2PartHi;
 __device__ __forceinline__ double table_exp(double x, const double* table) {
-  if (x < -700.0) return 0.0;
+  x = fmax(x, -700.0);
   const double k = rint(x * (64.0 / 0.693147180559945309417));
   const double r = fma(-k, kLn2PartLo, fma(-k, kLn2PartHi, x));
   double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
@@ -816,11 +856,19 @@ __device__ __noinline__ double row_sum(const SelectArgs& a, int32_t row, double 
   __syncthreads();
   const char* logits = a.logits + static_cast<int64_t>(row) * a.row_stride * E::kBytes;
   const RowMask mask = a.renormalize ? row_mask(a.masks, row) : RowMask{nullptr, nullptr};
+  // each thread the same tokens whatever the row's alignment, so that equal rows have equal sums
+  const bool aligned = (reinterpret_cast<uintptr_t>(logits) & 15u) == 0;
+  const int32_t vecs = (a.vocab + E::kPer - 1) / E::kPer;
   double sum = 0.0;
-#pragma unroll 4
-  for (int32_t t = threadIdx.x; t < a.vocab; t += kMergeThreads) {
-    const double x = E::one(logits + static_cast<int64_t>(t) * E::kBytes);
-    if (mask.all() || ((mask.word(t >> 5) >> (t & 31)) & 1u)) sum += table_exp(x - ref, table);
+#pragma unroll 1
+  for (int32_t i = threadIdx.x; i < vecs; i += kMergeThreads) {
+    const int32_t t0 = i * E::kPer;
+    uint4 v = aligned ? load_vector<E>(logits, t0, a.vocab) : load_edge<E>(logits, t0, a.vocab);
+    if (!mask.all()) E::keep(v, mask.word(t0 >> 5) >> (t0 & 31) & ((1u << E::kPer) - 1u));
+    double part = 0.0;
+#pragma unroll 4  // more of them would take more registers than the kernel has, and slow every call
+    for (int32_t k = 0; k < E::kPer; ++k) part += table_exp(static_cast<double>(E::at(v, k)) - ref, table);
+    sum += part;
   }
 #pragma unroll
   for (int32_t d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
