@@ -512,6 +512,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
   constexpr int32_t kStepTokens = kScanWarps * kWarpTokens;
   constexpr uint32_t kAll = (1u << kPer) - 1u;
   constexpr bool kSkips = MASKED && RENORMALIZE;  // vectors without an allowed token are not read
+  static_assert(kRound % 8 == 0, "mask words are loaded eight steps at a time");
   static_assert(kVecs * kPer <= 32, "a lane's bits of a step fit one word");
   const SelectArgs& a = s.a;
   const int32_t row = blockIdx.x / s.shares, share = blockIdx.x - row * s.shares;
@@ -527,15 +528,35 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
   // the warp's first token of a step; a lane's vectors follow one another at 32 vectors' distance
   const auto warp_token = [&](int32_t step) { return step * kStepTokens + warp * kWarpTokens - head; };
   const RowMask mask = MASKED ? row_mask(a.masks, row) : RowMask{nullptr, nullptr};
-  // the mask word that the lane holds of the warp's tokens of a step (aligned rows; tokens past
-  // the row cleared), and from the lanes' words each lane's own bits, kPer a vector
-  const auto load_word = [&](int32_t step) {
-    if (!MASKED || head != 0 || step >= end || lane * 32 >= kWarpTokens) return 0u;
-    const int32_t w = warp_token(step) / 32 + lane, left = vocab - w * 32;
-    if (left <= 0) return 0u;
-    const uint32_t word = mask.all() ? kFull : mask.word(w);
-    return left < 32 ? word & ((1u << left) - 1u) : word;
+  // The mask words that the lanes hold of the warp's tokens, `kWords` steps from `step` on
+  // (aligned rows; tokens past the row cleared), into the table, where the steps' maxima will lie.
+  // The loads come before the first store: a store waits for its own load.
+  constexpr int32_t kWords = 8;
+  const auto load_words = [&](int32_t step, int32_t stop, uint32_t* to) {
+    uint32_t got[kWords];
+    const int32_t w0 = (step * kStepTokens + warp * kWarpTokens) / 32 + lane;
+    const int32_t steps = lane * 32 < kWarpTokens ? stop - step : 0;
+    const uint32_t* words = mask.base ? mask.base : mask.delta;
+    const uint32_t* more = mask.base ? mask.delta : nullptr;
+#pragma unroll
+    for (int32_t k = 0; k < kWords; ++k) {
+      const int32_t w = w0 + k * (kStepTokens / 32);
+      got[k] = k < steps && w * 32 < vocab ? words ? words[w] : kFull : 0u;
+    }
+    if (more) {
+#pragma unroll
+      for (int32_t k = 0; k < kWords; ++k) {
+        const int32_t w = w0 + k * (kStepTokens / 32);
+        if (k < steps && w * 32 < vocab) got[k] |= more[w];
+      }
+    }
+#pragma unroll
+    for (int32_t k = 0; k < kWords; ++k) {
+      const int32_t left = vocab - (w0 + k * (kStepTokens / 32)) * 32;
+      to[k * kScanThreads] = left > 0 && left < 32 ? got[k] & ((1u << left) - 1u) : got[k];
+    }
   };
+  // from the lanes' words each lane's own bits, kPer a vector
   const auto own_bits = [&](int32_t step, uint32_t word) {
     uint32_t bits = 0u;
     if (head == 0) {
@@ -591,10 +612,10 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
     uint32_t bits[kSteps] = {0u, 0u};
     if (MASKED) {
       if (!scans) return;
-      // the round's mask words, all in flight together: a step's lie where its maxima will
-#pragma unroll 8
-      for (int32_t k = 0; k < kRound; ++k)
-        if (round + k < stop) sh.tops[k][tid] = load_word(round + k);
+      if (head == 0) {
+#pragma unroll 1
+        for (int32_t k = 0; k < kRound && round + k < stop; k += kWords) load_words(round + k, stop, &sh.tops[k][tid]);
+      }
       bits[0] = own_bits(round, sh.tops[0][tid]);
       if (round + 1 < stop) bits[1] = own_bits(round + 1, sh.tops[1][tid]);
     }
