@@ -27,6 +27,15 @@ constexpr uint32_t kFull = 0xffffffffu;
 // Each logit is read once: a step adds its exponentials to the thread's sum and leaves the
 // maximum of the thread's vectors in shared memory.  The best tokens lie in the few entries of
 // that table whose maximum is among its best; those alone are read again for their tokens.
+// (Listing candidate vectors against a running bound instead cost a barrier a step and, in most
+// warp-steps, a divergent push: 31 us against 25 for 256 rows of 128,256 bf16.)
+//
+// What bounds it: a CTA's fixed way -- flags, mask words, first data, then the bound, the entries
+// and their tokens, some 7 us of latencies -- around its stream, which runs at the SM's share of
+// the memory rate.  256 rows of 128,256 bf16 (a fifth of them ended, 52 MB): both kernels 23.3 us
+// where the bytes take 8.0; the stream is 8 of them, the exponentials' unit 3, the launches and
+// the merge 6.  Masked rows are also bound by instructions where a mask is mixed (the bits' spread
+// and the blend): 27.9 us, 5.8 for the bytes.
 
 constexpr int32_t kScanThreads = 256;
 constexpr int32_t kScanWarps = kScanThreads / 32;
@@ -36,7 +45,7 @@ constexpr int32_t kRound = 16;        // steps of the table; after as many the b
 constexpr int32_t kListCap = 512;     // entries read again; see list_crowded for why they suffice
 constexpr int32_t kPushCap = 1024;    // tokens (keys) of the listed entries
 constexpr int32_t kRankMost = kScanThreads;  // keys put in order by counting
-constexpr float kFar = 65536.0f;
+constexpr float kFar = 65536.0f;      // logits of this magnitude take the difference from the maximum first
 constexpr int32_t kPoolMax = 8192;    // candidates of a group that the second kernel takes
 
 // Floats as unsigned integers of the same order (-0 made +0 by the caller).
@@ -194,7 +203,7 @@ __device__ __forceinline__ RowMask row_mask(const RowMasks& m, int32_t row) {
 // first (rising(logit) << 32 | ~token; 0: none).
 struct Part {
   double sum;      // of 2^(x log2 e - anchor)
-  double far_sum;  // of exp(x - far), from tiles whose maximum is far from 0
+  double far_sum;  // of exp(x - far), from steps whose maximum is far from 0
   float anchor;    // a whole number; -inf: no sum
   float far;       // -inf: no far sum
 };
@@ -203,7 +212,7 @@ struct ScanArgs {
   SelectArgs a;
   Part* parts;      // [rows][shares]
   uint64_t* keys;   // [rows][shares][candidates]
-  int32_t shares, tiles_per_share;
+  int32_t shares, steps_per_share;
   int32_t pool;     // beams * shares * candidates
 };
 
@@ -522,8 +531,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
   const char* logits = a.logits + static_cast<int64_t>(row) * a.row_stride * E::kBytes;
   // vectors start at 16-byte boundaries, so the first may begin before the row
   const int32_t head = static_cast<int32_t>(reinterpret_cast<uintptr_t>(logits) & 15u) / E::kBytes;
-  const int32_t begin = share * s.tiles_per_share;
-  const int32_t end = min(begin + s.tiles_per_share, (vocab + head + kStepTokens - 1) / kStepTokens);
+  const int32_t begin = share * s.steps_per_share;
+  const int32_t end = min(begin + s.steps_per_share, (vocab + head + kStepTokens - 1) / kStepTokens);
 
   // the warp's first token of a step; a lane's vectors follow one another at 32 vectors' distance
   const auto warp_token = [&](int32_t step) { return step * kStepTokens + warp * kWarpTokens - head; };
@@ -819,7 +828,10 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
 
 // ---------------------------------------------------------------------------------------
 // Selection, second kernel: one CTA per group scores the rows' candidates in 64 bits and
-// orders the best.
+// orders the best: 4 us of latencies (loads, a logarithm, four barriers) behind a launch that
+// overlaps the scan's end.  Above kDirect candidates a histogram of their distances from the best
+// leaves few to put in order (a bisection of their bits took 11 us where this takes 7, and a
+// sample's bound kept hundreds where beams' scores differ: 26 us).
 
 constexpr int32_t kMergeThreads = 512;
 constexpr int32_t kMergeWarps = kMergeThreads / 32;
@@ -827,7 +839,11 @@ constexpr int32_t kMergeKeys = 4;    // keys that a thread loads ahead
 constexpr int32_t kDirect = 128;     // so many candidates are put in order without a selection before
 constexpr int32_t kBuckets = 512;    // of 1/16 of a score's unit each
 constexpr double kLn2 = 0.693147180559945309417;
-// Two beams' candidates nearer than this are ordered by log-sums taken again in 64 bits.
+// Two beams' candidates nearer than this are ordered by log-sums taken again in 64 bits.  The
+// scan's sums are within 3.1e-7 of the 64-bit ones (measured: 24 kinds of rows of 300 to 128,256
+// logits, constant, flat, peaked and shifted ones among them, 256 of each and of each type), so
+// the difference of two is within 6.2e-7.  Two beams come this near in about one call in fifty of
+// 32 groups, whose merge then takes about 40 us a row more.
 constexpr double kNear = 1e-6;
 
 struct MergeShared {
@@ -1312,6 +1328,11 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
 // parents form, a parent is read once however many children it has, and rows that stay are not
 // touched.  A thread fills its slots with as many units as they hold at a time; the CTAs of an
 // SM overlap one's loads with another's stores.
+//
+// Bound by memory: 963 MB of moves (8 caches of 256 rows, ragged lengths) in 151 us, 97% of the
+// copy rate; one request's 48 tensors, 165 MB, in 31 us (81%: a CTA's start, with the read of its
+// parents, shows).  Units held in registers took 167 and 79 us (a row's addresses and units a
+// thread leave few threads), CTAs that walk all tensors 178 and 56.
 
 constexpr int32_t kMoveThreads = 128;
 constexpr int32_t kMoveSlots = 24;    // 16-byte slots of a thread (or one per beam, if more)
@@ -1547,6 +1568,10 @@ __device__ __forceinline__ void copy_word_async(void* shared, const void* global
 // beam at the window's end of each last place, and a second walk of the segments every step's
 // beam, by which the tokens are picked.  So the walk is 2 * segment + segments + cluster links
 // long instead of the steps', and the rest is loads and stores side by side.
+//
+// Bound by that chain of latencies: 32 groups x 8 beams x 1,024 steps 7.6 us, 64 x 32 x 2,048 (35
+// MB with the output) 19.5 us, of which the first loads are 4, the two walks 3 and the cluster's
+// waits for its slowest CTA about 4; one CTA a group and one load at a time took 14 and 88.
 __global__ void __launch_bounds__(kTraceThreads, 4) trace_kernel(const __grid_constant__ TraceArgs a) {
   extern __shared__ __align__(16) uint8_t shared[];
   const int32_t beams = a.beams, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1697,7 +1722,7 @@ int sm_count(int32_t* out) {
 }
 
 struct Plan {
-  int32_t shares, tiles_per_share, pool;
+  int32_t shares, steps_per_share, pool;
   int64_t bytes;
 };
 
@@ -1728,8 +1753,8 @@ int plan(int32_t groups, int32_t beams, int32_t vocab, int32_t dtype, int32_t ca
   if (shares > kPoolMax / (beams * candidates)) shares = kPoolMax / (beams * candidates);
   if (shares > tiles) shares = tiles;
   if (shares < 1) shares = 1;
-  out->tiles_per_share = static_cast<int32_t>((tiles + shares - 1) / shares);
-  out->shares = (tiles + out->tiles_per_share - 1) / out->tiles_per_share;
+  out->steps_per_share = static_cast<int32_t>((tiles + shares - 1) / shares);
+  out->shares = (tiles + out->steps_per_share - 1) / out->steps_per_share;
   out->pool = beams * out->shares * candidates;
   out->bytes = rows * out->shares * (static_cast<int64_t>(sizeof(Part)) + candidates * static_cast<int64_t>(sizeof(uint64_t)));
   return XG_OK;
@@ -1787,7 +1812,7 @@ int select(const SelectArgs& a, cudaStream_t stream) {
   s.parts = reinterpret_cast<Part*>(a.workspace);
   s.keys = reinterpret_cast<uint64_t*>(a.workspace + parts * static_cast<int64_t>(sizeof(Part)));
   s.shares = p.shares;
-  s.tiles_per_share = p.tiles_per_share;
+  s.steps_per_share = p.steps_per_share;
   s.pool = p.pool;
   if (a.dtype == XG_F32) return launch_select<F32>(s, stream);
   if (a.dtype == XG_BF16) return launch_select<BF16>(s, stream);
