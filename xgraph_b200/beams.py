@@ -246,12 +246,11 @@ def _row_tensors(tensors, dim, device) -> tuple[bytes, int]:
     kind, first = _torch.Tensor, tensors[0]
     if not isinstance(first, kind):
         raise ValueError("tensors must be torch tensors")
-    shape, stride, count, dtype, index = first.shape, first.stride(), first.numel(), first.dtype, device.index
-    # one shape and type for all, without gaps, as a model's layers have: one layout serves (equal
-    # strides and sizes of tensors without gaps are equal shapes)
+    shape, dtype, index = first.shape, first.dtype, device.index
+    # one shape and type for all, without gaps, as a model's layers have: one layout serves
     if not isinstance(dim, list) and set(map(type, tensors)) == {kind} and all(
-            [t.is_contiguous() and t.stride() == stride and t.numel() == count and t.dtype == dtype
-             and t.get_device() == index and not t.requires_grad for t in tensors]):
+            [t.is_contiguous() and t.shape == shape and t.dtype == dtype and t.get_device() == index
+             and not t.requires_grad for t in tensors]):
         layout, size, _ = _layout(first, dim, device)
         places = [t.data_ptr() for t in tensors]
         if len(places) > 1 and size:
