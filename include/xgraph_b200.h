@@ -430,7 +430,8 @@ XG_API int xg_beam_workspace(int32_t groups, int32_t beams, int32_t vocab, int32
  * that is not finite (a NaN or +inf logit in N_r).  Places left over hold score -inf, beam
  * and token -1.  A candidate's float32 score is rounded once from 64 bits; the order is by
  * 64-bit scores, whose log-sum is taken again in 64 bits where two beams' candidates lie
- * within the 32-bit sum's error of each other. */
+ * within the 32-bit sum's error of each other.  (Two unequal logits of one beam so close, or
+ * beside a score so large, that their 64-bit scores are equal: either may be offered first.) */
 XG_API int xg_beam_select(const void* logits, int32_t dtype, int32_t groups, int32_t beams, int32_t vocab,
                           int64_t row_stride, const float* scores, const uint32_t* mask, int64_t mask_stride,
                           const uint8_t* finished, int32_t candidates, int32_t end_token, int32_t renormalize,
@@ -438,7 +439,8 @@ XG_API int xg_beam_select(const void* logits, int32_t dtype, int32_t groups, int
                           void* workspace, int64_t workspace_bytes, void* stream);
 /* xg_beam_select under the engine's own masks, read in place (nothing is written into the
  * logits): row r belongs to slots[r] (device int32 [groups * beams]); rows of inactive slots
- * and of slots in the error phase take every token < vocab, as apply_mask leaves them.
+ * and of slots in the error phase take every token < vocab, as apply_mask leaves them; vocab,
+ * the workspace's too, is the lesser of cols and the engine's.
  * XG_EINVAL for an engine with a logit policy (release or escape bias), whose rows only
  * xg_apply_mask and the fused step produce. */
 XG_API int xg_engine_beam_select(XgEngine* engine, const void* logits, int32_t dtype, int32_t groups, int32_t beams,
@@ -463,8 +465,8 @@ typedef struct XgRowTensor {
  * g * beams + b), at positions below lengths[g] of the tensor's position_dim (lengths:
  * device int32 [groups], or null: whole rows); every other position keeps its value.  A
  * parent outside [0, beams) leaves its row as it is, and so does a row number outside the
- * tensor.  Tensors must not overlap one another or themselves; the host descriptors are
- * read before the call returns. */
+ * tensor.  Tensors must not overlap one another, themselves or the three tables; the host
+ * descriptors are read before the call returns. */
 XG_API int xg_beam_reorder(const XgRowTensor* tensors, int32_t count, const int32_t* parents, int32_t groups,
                            int32_t beams, const int32_t* lengths, const int32_t* rows, void* stream);
 /* The same for the engine's slots: slots[g][b] takes the whole state of slots[g][parents[g][b]]

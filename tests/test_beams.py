@@ -101,6 +101,15 @@ def test_reorder_refusals(tensor, message, lengths):
     refused(lib.xg_beam_reorder(records(GOOD), 1, FAKE, 70000, 4, None, None, None), "groups")
 
 
+@pytest.mark.parametrize("tables", [(1 << 20, None, None), ((1 << 20) + 8 * 240 - 4, None, None),
+                                    ((1 << 20) - 28, None, None), (1, 1 << 20, None), (1, None, (1 << 20) + 100)])
+def test_reorder_refuses_tables_inside_a_tensor(tables):
+    """The parents, lengths or rows would change while they are read."""
+    parents, lengths, rows = (ctypes.c_void_p(t) if t else None for t in tables)
+    given = records((*GOOD[:5], 0, 1 << 24), (*GOOD[:5], 0))
+    refused(library().xg_beam_reorder(given, 2, parents, 2, 4, lengths, rows, None), "share memory")
+
+
 def test_null_engine():
     lib = library()
     refused(lib.xg_reorder_slots(None, FAKE, FAKE, 1, 4, None), "null engine")

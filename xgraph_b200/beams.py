@@ -103,7 +103,8 @@ def beam_select(logits, scores, *, mask=None, finished=None, candidates: int | N
     `finished` (bool [groups, beams]) marks beams that have ended: each offers one
     continuation, end_token, at its own score.  A continuation has ended when its beam had or
     its token is end_token.  Order: the score in 64 bits, equal scores by the lower (beam,
-    token).  A beam of score -inf is empty (start a search with scores [0, -inf, ...]); a beam
+    token); of a beam's unequal logits that 64 bits score alike, either may be offered first.
+    A beam of score -inf is empty (start a search with scores [0, -inf, ...]); a beam
     of NaN or +inf score, or whose logits hold a NaN or +inf that counts, offers nothing, and
     so does one that may take no token.
     """
@@ -209,7 +210,8 @@ def beam_reorder(tensors, beams, *, lengths=None, dim: int | Sequence[int] | Non
 
     With lengths [groups] int32 only the positions below lengths[group] of dimension `dim` of
     each tensor move (one dimension for all or one per tensor), such as the written part of a
-    cache; everything else keeps its value.  Tensors must not share memory.
+    cache; everything else keeps its value.  Tensors must not share memory, also not with
+    beams, lengths and rows.
     """
     torch = _load()
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)

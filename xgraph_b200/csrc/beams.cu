@@ -1917,6 +1917,18 @@ int describe(const XgRowTensor& t, bool has_lengths, MoveTensor* out, bool* empt
   return XG_OK;
 }
 
+// A table of n words lies in a (described) tensor without gaps: the move would change it while it is read.
+bool holds(const XgRowTensor& t, const int32_t* table, int64_t n) {
+  if (!table || t.rows == 0) return false;
+  int64_t elements = t.rows, extent = 1 + (t.rows - 1) * t.row_stride;
+  for (int32_t k = 0; k < t.dims; ++k) {
+    elements *= t.size[k];
+    extent += (t.size[k] - 1) * t.stride[k];
+  }
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(t.data), at = reinterpret_cast<uintptr_t>(table);
+  return elements > 0 && elements == extent && at < begin + extent * t.element_bytes && begin < at + n * sizeof(int32_t);
+}
+
 int launch_moves(const MoveArgs& a, int64_t most_units, cudaStream_t stream) {
   int32_t sms = 0;
   if (int rc = sm_count(&sms)) return rc;
@@ -1953,7 +1965,12 @@ int reorder(const XgRowTensor* tensors, int32_t count, const int32_t* parents, i
   a.parents = parents;
   a.lengths = lengths;
   a.row_of = rows;
+  const int64_t places = static_cast<int64_t>(groups) * beams;
   for (int32_t launches = 0; launches < 2; ++launches) {  // every descriptor is checked before the first launch
+    if (launches)
+      for (int32_t k = 0; k < count; ++k)
+        if (holds(tensors[k], parents, places) || holds(tensors[k], lengths, groups) || holds(tensors[k], rows, places))
+          return fail(XG_EINVAL, "parents, lengths and rows must not share memory with a tensor that is moved");
     a.count = 0;
     int64_t most_units = 0;
     for (int32_t k = 0; k < count; ++k) {

@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes
 import math
 from collections.abc import Iterable
+from contextlib import nullcontext
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -661,19 +662,23 @@ class Engine:
         cursor, STOP table).  Both int32 [groups, beams]; slots distinct; an entry of beams
         outside [0, beams) leaves its slot as it is.  The next sync reads each slot's history
         from the cursor it took over, so a slot's history row needs its new tokens only."""
-        import torch
+        from . import beams as _beams
 
+        torch = _beams._load()
         for name, table in (("slots", slots), ("beams", beams)):
             if (not isinstance(table, torch.Tensor) or not table.is_cuda or table.dtype != torch.int32
                     or table.dim() != 2 or not table.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous [groups, beams] int32 tensor on the GPU")
+            if table.device.index != self._info.device:
+                raise ValueError(f"{name} must be on the engine's GPU (cuda:{self._info.device})")
         if slots.shape != beams.shape:
             raise ValueError("slots and beams must have the same shape")
         if slots.numel() > self.max_sequences:
             raise ValueError("more slots than max_sequences")
-        _check(self._lib.xg_reorder_slots(self._handle, ctypes.c_void_p(slots.data_ptr()),
-                                          ctypes.c_void_p(beams.data_ptr()), slots.shape[0], slots.shape[1],
-                                          _stream(stream)))
+        with _beams._placed(self._info.device, stream) or nullcontext():
+            _check(self._lib.xg_reorder_slots(self._handle, ctypes.c_void_p(slots.data_ptr()),
+                                              ctypes.c_void_p(beams.data_ptr()), slots.shape[0], slots.shape[1],
+                                              _stream(stream)))
 
     def _row_slots(self, row_slots, name="row_slots"):
         import torch
