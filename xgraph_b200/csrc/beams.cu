@@ -63,7 +63,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-__device__ __forceinline__ float exp2_fast(float x) {  // within 2 units of 2^-23 of 2^x
+__device__ __forceinline__ float exp2_fast(float x) {  // within 2^-22 of 2^x, relatively
   float d;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
   return d;
@@ -86,6 +86,10 @@ __device__ __forceinline__ float high(uint64_t a) { return __uint_as_float(stati
 
 constexpr float kLog2eHi = 1.44269502162933349609375f;  // log2(e) in two floats
 constexpr float kLog2eLo = 1.92596299112661746887e-8f;
+// An anchor's natural logarithm: sums are of 2^(x kLog2eHi - anchor), so of exp(x - ref), nearly,
+// with the ref at which x kLog2eHi is the anchor.
+constexpr double kAnchorLn = 1.0 / static_cast<double>(kLog2eHi);
+constexpr float kAbove = 8.0f;  // a warp's maximum stands up to this much above its anchor
 
 // How the three logit types sit in a 16-byte vector.
 struct F32 {
@@ -202,7 +206,7 @@ __device__ __forceinline__ RowMask row_mask(const RowMasks& m, int32_t row) {
 // What the scan leaves for the merge: per (row, share) the sum's parts, and its best keys, best
 // first (rising(logit) << 32 | ~token; 0: none).
 struct Part {
-  double sum;      // of 2^(x log2 e - anchor)
+  double sum;      // of 2^(x kLog2eHi - anchor)
   double far_sum;  // of exp(x - far), from steps whose maximum is far from 0
   float anchor;    // a whole number; -inf: no sum
   float far;       // -inf: no far sum
@@ -673,11 +677,11 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
         if (!isfinite(most)) {
           if (anchor == -CUDART_INF_F) anchor = 0.0f;  // whatever the anchor, the sum will show it
         } else if (fabsf(most) < kFar) {
-          const float near = ceilf(most * kLog2eHi);
+          const float near = ceilf(most * kLog2eHi) - kAbove;
           if (near > anchor) {
             sum = anchor == -CUDART_INF_F ? 0.0 : sum * power2(anchor - near);
             anchor = near;
-            limit = near * 0.693147f;
+            limit = (near + kAbove) * 0.693147f;
           }
         } else {
           far_step = true;
@@ -685,36 +689,42 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_kernel(const __grid_cons
       }
       if (far_step) {  // so far from 0 that log2 e's rounding would show: the difference comes first
         const float most = from_rising(__reduce_max_sync(kFull, rising(shown)));
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        double part = 0.0;
 #pragma unroll 1
         for (int32_t j = 0; j < kVecs; ++j) {
           uint4 x = slot[j * kScanThreads];
           if (kSkips) E::keep(x, (own >> (j * kPer)) & kAll);
+          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int32_t k = 0; k < kPer; ++k) {
             const float d = E::at(x, k) - most;
             acc[k & 3] += exp2_fast(fmaf(d, kLog2eHi, d * kLog2eLo));
           }
+          part += static_cast<double>((acc[0] + acc[1]) + (acc[2] + acc[3]));
         }
-        const double part = static_cast<double>((acc[0] + acc[1]) + (acc[2] + acc[3]));
         const float higher = fmaxf(far, most);
         far_sum = (far == -CUDART_INF_F ? 0.0 : far_sum * exp_apart(static_cast<double>(far) - static_cast<double>(higher))) +
                   part * exp_apart(static_cast<double>(most) - static_cast<double>(higher));
         far = higher;
       } else if (anchor != -CUDART_INF_F) {
-        // exp(x) as 2^(x log2 e - anchor) with a whole anchor near the maximum: sums of
-        // different anchors differ by exact powers of two
-        const uint64_t hi = pack2(kLog2eHi, kLog2eHi), lo = pack2(kLog2eLo, kLog2eLo), back = pack2(-anchor, -anchor);
+        // exp(x) as 2^(x kLog2eHi - anchor) with a whole anchor near the maximum: sums of
+        // different anchors differ by exact powers of two.  Five additions deep (see kNear).
+        const uint64_t hi = pack2(kLog2eHi, kLog2eHi), back = pack2(-anchor, -anchor);
         uint64_t acc[2] = {0, 0};
 #pragma unroll
         for (int32_t j = 0; j < kVecs; ++j) {
           if (kSkips && !whole && !__any_sync(kFull, (own >> (j * kPer)) & kAll)) continue;
+          uint64_t e[kPer / 2];
 #pragma unroll
           for (int32_t k = 0; k < kPer; k += 2) {
-            const uint64_t x = pack2(E::at(v[j], k), E::at(v[j], k + 1));
-            const uint64_t y = fma2(x, lo, fma2(x, hi, back));
-            acc[(k >> 1) & 1] = add2(acc[(k >> 1) & 1], pack2(exp2_fast(low(y)), exp2_fast(high(y))));
+            const uint64_t y = fma2(pack2(E::at(v[j], k), E::at(v[j], k + 1)), hi, back);
+            e[k >> 1] = pack2(exp2_fast(low(y)), exp2_fast(high(y)));
           }
+#pragma unroll
+          for (int32_t n = kPer / 4; n > 0; n >>= 1)
+#pragma unroll
+            for (int32_t k = 0; k < n; ++k) e[k] = add2(e[k], e[k + n]);
+          acc[j & 1] = add2(acc[j & 1], e[0]);
         }
         const uint64_t all = add2(acc[0], acc[1]);
         sum += static_cast<double>(low(all) + high(all));
@@ -838,13 +848,24 @@ constexpr int32_t kMergeWarps = kMergeThreads / 32;
 constexpr int32_t kMergeKeys = 4;    // keys that a thread loads ahead
 constexpr int32_t kDirect = 128;     // so many candidates are put in order without a selection before
 constexpr int32_t kBuckets = 512;    // of 1/16 of a score's unit each
-constexpr double kLn2 = 0.693147180559945309417;
-// Two beams' candidates nearer than this are ordered by log-sums taken again in 64 bits.  The
-// scan's sums are within 3.1e-7 of the 64-bit ones (measured: 24 kinds of rows of 300 to 128,256
-// logits, constant, flat, peaked and shifted ones among them, 256 of each and of each type), so
-// the difference of two is within 6.2e-7.  Two beams come this near in about one call in fifty of
-// 32 groups, whose merge then takes about 40 us a row more.
-constexpr double kNear = 1e-6;
+// Two beams' candidates nearer than this are ordered by log-sums taken again in 64 bits.  A scan's
+// log-sum is within 9.8e-7 of the exact one, so the difference of two is within 1.96e-6.  A warp's
+// terms are 2^y, y = x kLog2eHi - anchor, whose largest lies in (kAbove - 1, kAbove] = (7, 8] (give
+// or take 0.03 by rounding); a sum's relative error is the mean of its terms' errors by weight:
+//   3.4e-7  y is rounded once: by 2^-21 at most while |y| < 16, which moves 2^y by 2^-21 ln 2.  A warp
+//           takes up to 2^17 tokens (2^20 on 8 warps), so those at y <= -16 weigh 2^17 2^-16 / 2^7 at
+//           most and add 1e-8;
+//   1.0e-7  log2 e is taken as kLog2eHi, 1.34e-8 of it too small: a term moves by that times |x - ref|
+//           (in the natural unit), whose mean by weight is within 10 ln 2: at the upper end y <= 8, at
+//           the lower an entropy bounds it, -mean(y) <= log2(2^17) - log2(2^7) = 10;
+//   2.4e-7  the exponential, 2^-22 (its documented bound);
+//   3.0e-7  five 32-bit additions from a term to the 64-bit sum, 2^-24 each.
+// Steps far from zero (kFar) stand below these: their y reaches 0 and not 8, but 2^10 tokens share a
+// maximum, x - most is exact wherever it counts, both parts of log2 e are taken and the additions are
+// three deep.  Merging is in 64 bits by exact powers of two.
+// Two beams come this near in about one call in twenty-five of 32 groups, whose merge then takes
+// about 40 us a row more.
+constexpr double kNear = 2e-6;
 
 struct MergeShared {
   double log_sum[kMaxBeams];   // log of the row's sum of exp(x - ref)
@@ -1156,7 +1177,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
         }
         p = total_part(p, width);
         double sum = p.sum;
-        ref = p.anchor == -CUDART_INF_F ? 0.0 : static_cast<double>(p.anchor) * kLn2;
+        ref = p.anchor == -CUDART_INF_F ? 0.0 : static_cast<double>(p.anchor) * kAnchorLn;
         if (p.far != -CUDART_INF_F) {
           const double far = static_cast<double>(p.far);
           const double higher = p.anchor == -CUDART_INF_F || far > ref ? far : ref;
