@@ -1852,7 +1852,6 @@ struct Dim {
 // dimension's outer side, whose extent differs by group).
 int describe(const XgRowTensor& t, bool has_lengths, MoveTensor* out, bool* empty) {
   const int32_t e = t.element_bytes;
-  if (!t.data) return fail(XG_EINVAL, "null tensor");
   if (e != 1 && e != 2 && e != 4 && e != 8 && e != 16) return fail(XG_EINVAL, "elements must have 1, 2, 4, 8 or 16 bytes");
   if (t.dims < 0 || t.dims > 4) return fail(XG_EINVAL, "a row has at most 4 dimensions");
   if (t.position_dim < -1 || t.position_dim >= t.dims || (has_lengths && t.position_dim < 0))
@@ -1861,7 +1860,7 @@ int describe(const XgRowTensor& t, bool has_lengths, MoveTensor* out, bool* empt
   Dim d[4];
   int32_t n = 0;
   bool single = false;  // the position dimension has one place: a row moves if its length is not 0
-  *empty = false;
+  *empty = t.rows == 0;
   for (int32_t k = 0; k < t.dims; ++k) {
     if (t.size[k] < 0) return fail(XG_EINVAL, "negative size");
     if (t.size[k] == 0) *empty = true;
@@ -1873,7 +1872,8 @@ int describe(const XgRowTensor& t, bool has_lengths, MoveTensor* out, bool* empt
     }
     d[n++] = Dim{t.size[k], t.stride[k] * e, position};
   }
-  if (*empty) return XG_OK;
+  if (*empty) return XG_OK;  // nothing to move, whatever the address: such tensors have none
+  if (!t.data) return fail(XG_EINVAL, "null tensor");
   for (int32_t i = 1; i < n; ++i)  // the largest stride first: the order of a row's dimensions is free
     for (int32_t j = i; j > 0 && d[j].stride > d[j - 1].stride; --j) {
       const Dim x = d[j];
