@@ -62,9 +62,10 @@ def _load():
 
         from .engine import _check, load_library
 
-        _lib, _call_errors, _torch = load_library(), _check, torch
+        _call_errors, _torch = _check, torch
         _get_device, _get_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
         _dtypes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+        _lib = load_library()  # last: another thread's first call may see it and go on
     return _torch
 
 
