@@ -31,6 +31,7 @@ from typing import NamedTuple
 MAX_BEAMS = 64
 MAX_CANDIDATES = 128
 MAX_BEAM_VOCAB = 1 << 20
+_INT32 = (1 << 31) - 1
 
 # XgRowTensor: data, then rows, row_stride, size[4], stride[4], dims, element_bytes, position_dim, reserved
 _ADDRESS, _ROW_LAYOUT = struct.Struct("<q"), struct.Struct("<qq4q4q4i")
@@ -89,6 +90,18 @@ def _table(tensor, name: str, shape, dtype, device):
     return tensor.data_ptr()
 
 
+def _check_sizes(groups: int, beams: int, vocab: int = 1, candidates: int = 1, steps: int = 0) -> None:
+    """The limits, before a size reaches the C entry points, which take the low 32 bits of it."""
+    if not 1 <= beams <= MAX_BEAMS:
+        raise ValueError(f"a group holds 1 to {MAX_BEAMS} beams, got {beams}")
+    if not 1 <= candidates <= MAX_CANDIDATES:
+        raise ValueError(f"candidates must be between 1 and {MAX_CANDIDATES}, got {candidates}")
+    if not 1 <= vocab <= MAX_BEAM_VOCAB:
+        raise ValueError(f"the vocabulary must hold 1 to {MAX_BEAM_VOCAB} tokens, got {vocab}")
+    if groups > _INT32 or steps > _INT32:
+        raise ValueError(f"too many {'groups' if groups > _INT32 else 'steps'}")
+
+
 def beam_select(logits, scores, *, mask=None, finished=None, candidates: int | None = None, vocab: int | None = None,
                 end_token: int | None = None, renormalize: bool = True, stream: int = 0) -> BeamCandidates:
     """The `candidates` best continuations of each group (default: as many as beams).
@@ -140,6 +153,7 @@ def _select(engine, logits, slots, scores, mask, finished, candidates, vocab, en
     elif not 1 <= vocab <= columns:
         raise ValueError(f"vocab must be between 1 and the {columns} columns, got {vocab}")
     wanted = beams if candidates is None else int(candidates)
+    _check_sizes(groups, beams, vocab, wanted)
     mask_at, mask_stride = None, 0
     if mask is not None:
         if not isinstance(mask, torch.Tensor) or mask.dtype != torch.int32 or mask.device != device or mask.dim() != 2:
@@ -232,6 +246,7 @@ def beam_reorder(tensors, beams, *, lengths=None, dim: int | Sequence[int] | Non
         rows_at = _table(rows, "rows", (groups, per_group), torch.int32, device)
     if not tensors:
         return
+    _check_sizes(groups, per_group)
     if dim is not None and not isinstance(dim, int):
         dim = list(dim)
         if len(dim) != len(tensors):
@@ -332,6 +347,7 @@ def beam_sequences(tokens, beams, *, lengths=None, pad_token: int = -1, stream: 
     if tokens.shape != beams.shape or tokens.device != beams.device:
         raise ValueError("tokens and beams must have the same shape and device")
     steps, groups, per_group = tokens.shape
+    _check_sizes(groups, per_group, steps=steps)
     device = tokens.device
     lengths_at = None if lengths is None else _table(lengths, "lengths", (groups,), torch.int32, device)
     if not -(1 << 31) <= pad_token < 1 << 31:
