@@ -428,10 +428,12 @@ XG_API int xg_beam_workspace(int32_t groups, int32_t beams, int32_t vocab, int32
  * finished or the token is end_token (-1: none; required with finished).  Rows that offer
  * nothing: a score that is not finite (-inf marks an empty beam), nothing in A_r, or a sum
  * that is not finite (a NaN or +inf logit in N_r).  Places left over hold score -inf, beam
- * and token -1.  A candidate's float32 score is rounded once from 64 bits; the order is by
- * 64-bit scores, whose log-sum is taken again in 64 bits where two beams' candidates lie
- * within the 32-bit sum's error of each other.  (Two unequal logits of one beam so close, or
- * beside a score so large, that their 64-bit scores are equal: either may be offered first.) */
+ * and token -1.  A float32 score is within half a unit in its last place, plus 1e-6, of the
+ * exact one: the log-sum's exponentials are taken in 32 bits, and where two beams' candidates
+ * lie nearer than two such errors both sums are taken again in 64 bits, so that the order is
+ * that of the 64-bit scores.  (The same row's score may therefore differ in its last bits with
+ * the batch that it is in.  Two unequal logits so close, or beside a score so large, that their
+ * 64-bit scores are equal: either may be offered first.)  The outputs are none of the inputs. */
 XG_API int xg_beam_select(const void* logits, int32_t dtype, int32_t groups, int32_t beams, int32_t vocab,
                           int64_t row_stride, const float* scores, const uint32_t* mask, int64_t mask_stride,
                           const uint8_t* finished, int32_t candidates, int32_t end_token, int32_t renormalize,

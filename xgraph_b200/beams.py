@@ -14,10 +14,12 @@ batch holds `groups` requests of `beams` beams; row r = group * beams + beam.  O
 logits are not written), and `Engine.reorder` moves the slots' constraint states.  Kernels and
 C entry points: csrc/beams.cu, include/xgraph_b200.h.  The reference has no counterpart.
 
-Every function takes `stream` (a raw cudaStream_t as int, 0 = default stream), enqueues its
-kernels there and does not wait; tensors are on one GPU and stay valid until the stream has
-passed the call.  Captured into a CUDA graph (stream = the capturing stream), a call keeps
-its own workspace in the graph's memory.
+Every function takes `stream` (a raw cudaStream_t as int, 0 = the default stream, as the engine's
+methods do, whatever torch's current stream is: under `torch.cuda.stream(s)` give
+`stream=s.cuda_stream`), enqueues its kernels there and does not wait; tensors are on one GPU and
+stay valid until the stream has passed the call.  Captured into a CUDA graph (stream = the
+capturing stream), a call keeps its own workspace in the graph's memory.  No gradient goes
+through these functions: results need none, whether or not the inputs do.
 """
 
 from __future__ import annotations
@@ -117,10 +119,13 @@ def beam_select(logits, scores, *, mask=None, finished=None, candidates: int | N
     `finished` (bool [groups, beams]) marks beams that have ended: each offers one
     continuation, end_token, at its own score.  A continuation has ended when its beam had or
     its token is end_token.  Order: the score in 64 bits, equal scores by the lower (beam,
-    token); of a beam's unequal logits that 64 bits score alike, either may be offered first.
+    token); of unequal logits that 64 bits score alike, either may be offered first.  The scores
+    returned are within half a float32 unit in the last place, plus 1e-6, of the exact ones, and
+    their last bits may differ with the batch that a row is in.
     A beam of score -inf is empty (start a search with scores [0, -inf, ...]); a beam
     of NaN or +inf score, or whose logits hold a NaN or +inf that counts, offers nothing, and
-    so does one that may take no token.
+    so does one that may take no token.  At most MAX_BEAMS beams, MAX_CANDIDATES candidates and
+    MAX_BEAM_VOCAB tokens.
     """
     _load()
     return _select(None, logits, None, scores, mask, finished, candidates, vocab, end_token, renormalize, stream)
@@ -226,7 +231,7 @@ def beam_reorder(tensors, beams, *, lengths=None, dim: int | Sequence[int] | Non
     With lengths [groups] int32 only the positions below lengths[group] of dimension `dim` of
     each tensor move (one dimension for all or one per tensor), such as the written part of a
     cache; everything else keeps its value.  Tensors must not share memory, also not with
-    beams, lengths and rows.
+    beams, lengths and rows; those without elements are left out.
     """
     torch = _load()
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)

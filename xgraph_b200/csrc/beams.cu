@@ -32,10 +32,10 @@ constexpr uint32_t kFull = 0xffffffffu;
 //
 // What bounds it: a CTA's fixed way -- flags, mask words, first data, then the bound, the entries
 // and their tokens, some 7 us of latencies -- around its stream, which runs at the SM's share of
-// the memory rate.  256 rows of 128,256 bf16 (a fifth of them ended, 52 MB): both kernels 23.3 us
+// the memory rate.  256 rows of 128,256 bf16 (a fifth of them ended, 52 MB): both kernels 23.2 us
 // where the bytes take 8.0; the stream is 8 of them, the exponentials' unit 3, the launches and
 // the merge 6.  Masked rows are also bound by instructions where a mask is mixed (the bits' spread
-// and the blend): 27.9 us, 5.8 for the bytes.
+// and the blend): 27.5 us, 5.8 for the bytes.
 
 constexpr int32_t kScanThreads = 256;
 constexpr int32_t kScanWarps = kScanThreads / 32;
@@ -863,8 +863,8 @@ constexpr int32_t kBuckets = 512;    // of 1/16 of a score's unit each
 // Steps far from zero (kFar) stand below these: their y reaches 0 and not 8, but 2^10 tokens share a
 // maximum, x - most is exact wherever it counts, both parts of log2 e are taken and the additions are
 // three deep.  Merging is in 64 bits by exact powers of two.
-// Two beams come this near in about one call in twenty-five of 32 groups, whose merge then takes
-// about 40 us a row more.
+// Random logits bring two beams this near in one call of 60 (32 groups of 16 beams, 32 candidates)
+// to 1,600 (8 beams, 8 candidates), whose merge then takes about 40 us a row more.
 constexpr double kNear = 2e-6;
 
 struct MergeShared {
